@@ -229,7 +229,7 @@ inline FastDiv make_fastdiv(uint32_t d) {
   while ((1ull << s) < d) ++s;
   return FastDiv{(uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
 }
-__device__ __forceinline__ uint32_t fdiv(uint32_t n, FastDiv f) {
+__host__ __device__ __forceinline__ uint32_t fdiv(uint32_t n, FastDiv f) {
   return (uint32_t)(((uint64_t)n * f.m) >> (31 + f.s));
 }
 

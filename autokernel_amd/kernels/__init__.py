@@ -4,6 +4,9 @@ Each module exposes KERNEL_TYPE and kernel_fn with the signature of the matching
 function, like the reference's kernels/*.py slot modules. The kernel_fns themselves live in
 kernels/host.py (the shape layer shared with the HuggingFace Kernels export), bound here to the
 ctypes-backed ops of kernels/_ops.py.
+
+Beside the nine stand the operators of serving from a paged K / V cache, which the reference does not have:
+kv_append and paged_attention.
 """
 from __future__ import annotations
 
@@ -11,16 +14,17 @@ from . import _ops, host
 
 host.bind(_ops)
 
-from . import (cross_entropy, flash_attention, fused_mlp, layernorm, matmul, reduce, rmsnorm,  # noqa: E402
-               rotary_embedding, softmax)
+from . import (cross_entropy, flash_attention, fused_mlp, kv_append, layernorm, matmul,  # noqa: E402
+               paged_attention, reduce, rmsnorm, rotary_embedding, softmax)
 
 MODULES = {m.KERNEL_TYPE: m for m in (matmul, softmax, layernorm, rmsnorm, flash_attention,
-                                      fused_mlp, cross_entropy, rotary_embedding, reduce)}
+                                      fused_mlp, cross_entropy, rotary_embedding, reduce,
+                                      kv_append, paged_attention)}
 KERNELS = {name: m.kernel_fn for name, m in MODULES.items()}
 
 
 def get(kernel_type: str):
-    """kernel_fn for a KERNEL_TYPE name (bench.py KERNEL_CONFIGS keys)."""
+    """kernel_fn for a KERNEL_TYPE name (bench.py KERNEL_CONFIGS keys, and the serving operators)."""
     try:
         return KERNELS[kernel_type]
     except KeyError:

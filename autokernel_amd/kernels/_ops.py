@@ -237,3 +237,51 @@ def flash_attn_fwd(o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
     _run("ak_flash_attn_fwd", q, lambda: dict(Q=tuple(q.shape), K=tuple(k.shape), dtype=q.dtype), code, q.data_ptr(),
          k.data_ptr(), v.data_ptr(), o.data_ptr(), B, Hq, Hkv, Sq, Sk, D, st[0], st[1], st[2], st[3],
          int(bool(causal)), float(sm_scale))
+
+
+_I64x2 = ctypes.c_int64 * 2
+
+
+def _paged_sizes(k_cache: torch.Tensor, page_table: torch.Tensor) -> tuple:
+    """(num_pages, page_size, max_pages, table_stride)"""
+    return (k_cache.shape[0], k_cache.shape[2], page_table.shape[1],
+            page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1])
+
+
+def kv_append(q_out: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.Tensor, q: torch.Tensor | None,
+              k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None,
+              page_table: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor, interleaved: bool) -> None:
+    """k, v [T, Hkv, D] to their slots of the caches [pages, Hkv, page_size, D]; k and q [T, Hq, D] rotated
+    by the fp32 rows of cos / sin [rows, rot_dim / 2] (None: no rotation)."""
+    T, Hkv, D = k.shape
+    rows, rot = (0, 0) if cos is None else (cos.shape[0], 2 * cos.shape[1])
+    none = _I64x2(0, 0)
+    st = [none if t is None else _I64x2(*t.stride()[:2]) for t in (q, k, v, q_out)]
+    _run("ak_kv_append", k, lambda: dict(k=tuple(k.shape), cache=tuple(k_cache.shape), dtype=k.dtype),
+         _code(k, "kv_append"), _lib.ptr(q), k.data_ptr(), v.data_ptr(), _lib.ptr(q_out), k_cache.data_ptr(),
+         v_cache.data_ptr(), _lib.ptr(cos), _lib.ptr(sin), page_table.data_ptr(), q_starts.data_ptr(),
+         kv_lens.data_ptr(), T, kv_lens.shape[0], 0 if q is None else q.shape[1], Hkv, D, rot, rows,
+         *_paged_sizes(k_cache, page_table), *st, _I64x3(*k_cache.stride()[:3]), _I64x3(*v_cache.stride()[:3]),
+         int(bool(interleaved)))
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace_bytes(dtype: int, T: int, B: int, Hq: int, Hkv: int, D: int, page: int, width: int) -> int:
+    return _lib.load().ak_paged_attn_workspace_bytes(dtype, T, B, Hq, Hkv, D, page, width)
+
+
+def paged_attn(o: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+               page_table: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor, sm_scale: float) -> None:
+    """Attention of q [T, Hq, D] over the caches [pages, Hkv, page_size, D] into o [T, Hq, D]."""
+    T, Hq, D = q.shape
+    B, Hkv = kv_lens.shape[0], k_cache.shape[1]
+    code = _code(q, "paged_attention")
+    sizes = _paged_sizes(k_cache, page_table)
+    # fp32 partials of key slices
+    nbytes = _paged_workspace_bytes(code, T, B, Hq, Hkv, D, sizes[1], sizes[2])
+    ws = torch.empty(nbytes // 4, device=q.device, dtype=torch.float32) if nbytes > 0 else None
+    _run("ak_paged_attn", q, lambda: dict(q=tuple(q.shape), cache=tuple(k_cache.shape), dtype=q.dtype), code,
+         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), page_table.data_ptr(),
+         q_starts.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, *sizes, _I64x2(*q.stride()[:2]),
+         _I64x3(*k_cache.stride()[:3]), _I64x3(*v_cache.stride()[:3]), _I64x2(*o.stride()[:2]), float(sm_scale),
+         _lib.ptr(ws), nbytes)

@@ -331,6 +331,62 @@ int ak_flash_attn_fwd_ws(int dtype, const void* Q, const void* K, const void* V,
                          int causal, float sm_scale, void* workspace, int64_t workspace_bytes,
                          hipStream_t stream);
 
+/*
+ * The paged cache of ak_kv_append and ak_paged_attn. K and V each live in num_pages pages of page_size
+ * slots, every slot one token's [Hkv, D]; element strides (page, head, slot) say how a page is laid out
+ * ([pages, Hkv, page_size, D] and [pages, page_size, Hkv, D] alike), the last dim is contiguous.
+ * A call's T rows are the sequences' new tokens one after another: sequence b has rows
+ * q_starts[b] .. q_starts[b + 1] - 1 (q_starts: int32 [B + 1], rising) and, these new tokens included,
+ * kv_lens[b] cached tokens (int32 [B]). So row t is at position kv_lens[b] - (q_starts[b + 1] - t), and
+ * position p is slot p % page_size of page page_table[b * table_stride + p / page_size] (int32
+ * [B][max_pages]). Rows outside every sequence (behind the last one in a padded batch) are neither read
+ * nor written. These three arrays are read by the kernels only: no launch depends on their values, so a
+ * captured graph may be replayed with new ones. Every page number is checked on the device. All counts
+ * and max_pages * page_size must stay below 2^31.
+ *
+ * ak_kv_append: row t's k and v [Hkv, D] go to its slot, q and k rotated on the way: the first rot_dim
+ * dims of each head turn by the fp32 rows cos_t[pos], sin_t[pos] ([table_rows, rot_dim / 2], dense), in
+ * pairs (2i, 2i + 1) (interleaved != 0, as ak_rope) or (i, i + rot_dim / 2); every product and sum is
+ * rounded in fp32, the result once to the element type. The other dims, and v, are copied. The rotated
+ * q [T, Hq, D] goes to q_out (which may be q itself). Hq = 0: no q. rot_dim = 0: no rotation (Hq = 0 then).
+ * Strides of q, k, v, q_out are (row, head) in elements. A row whose position is below zero or, when
+ * rotating, past table_rows writes no k and v, and its q comes out NaN; one whose page is not in the
+ * cache writes no k and v. Two rows with one slot (a page listed twice) leave either one's values there.
+ * D up to 256 (above: AK_EUNSUPPORTED).
+ * No counterpart in the reference, whose models recompute every position (models/llama_7b.py:67-82).
+ */
+int ak_kv_append(int dtype, const void* q, const void* k, const void* v, void* q_out, void* k_cache,
+                 void* v_cache, const float* cos_t, const float* sin_t, const int32_t* page_table,
+                 const int32_t* q_starts, const int32_t* kv_lens, int64_t T, int64_t B, int64_t Hq,
+                 int64_t Hkv, int64_t D, int64_t rot_dim, int64_t table_rows, int64_t num_pages,
+                 int64_t page_size, int64_t max_pages, int64_t table_stride, const int64_t* q_strides,
+                 const int64_t* k_strides, const int64_t* v_strides, const int64_t* q_out_strides,
+                 const int64_t* k_cache_strides, const int64_t* v_cache_strides, int interleaved,
+                 hipStream_t stream);
+
+/*
+ * Attention of the new tokens over the paged cache: O_t = softmax_j(q_t . K_j * sm_scale) V_j over the
+ * positions j up to row t's own (the new tokens' K and V are in the cache already, see ak_kv_append).
+ * q, o: [T, Hq, D] by (row, head) strides; query head h reads KV head h / (Hq / Hkv). sm_scale > 0.
+ * Any mix of single tokens and chunks. fp32 scores, softmax statistics and sums. What a row does not see
+ * (later tokens, slots past the sequence's end, infinities and NaN among them) has no influence on it.
+ * A row that sees nothing (position below zero) is zero. A row that sees a position whose page is not in
+ * the cache is NaN, and so are all rows of a sequence with kv_lens[b] > max_pages * page_size.
+ *   ak_paged_attn_workspace_bytes: bytes of workspace a call of these sizes needs (0: none); it holds fp32
+ *     partial results of key slices, added in a fixed order (deterministic). Calls that may overlap need
+ *     a workspace each.
+ *   ak_paged_attn: workspace 16-byte aligned, AK_EINVAL when it is too small.
+ * No counterpart in the reference: its attention reads dense K and V (reference.py:32-42).
+ */
+int64_t ak_paged_attn_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                      int64_t page_size, int64_t max_pages);
+int ak_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o,
+                  const int32_t* page_table, const int32_t* q_starts, const int32_t* kv_lens, int64_t T,
+                  int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
+                  int64_t max_pages, int64_t table_stride, const int64_t* q_strides,
+                  const int64_t* k_cache_strides, const int64_t* v_cache_strides, const int64_t* o_strides,
+                  float sm_scale, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
