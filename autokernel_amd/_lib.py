@@ -63,6 +63,7 @@ SIGNATURES: dict[str, list] = {
                              _pi64, _pi64, _pi64, _pi64, _i, _f, _p, _i64, _p],
     "ak_kv_append": [_i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, *[_i64] * 11,
                      _pi64, _pi64, _pi64, _pi64, _pi64, _pi64, _i, _p],
+    "ak_sample": [_i, _p, _p, _p, _i64, _i64, _i64, _p, _f, _p, ctypes.c_int32, _p, _f, _p, _f, _p],
     "ak_paged_attn_workspace_bytes": [_i, *[_i64] * 7],
     "ak_paged_attn": [_i, _p, _p, _p, _p, _p, _p, _p, *[_i64] * 9, _pi64, _pi64, _pi64, _pi64, _f, _p, _i64, _p],
 }

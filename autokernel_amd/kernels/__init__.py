@@ -6,7 +6,7 @@ kernels/host.py (the shape layer shared with the HuggingFace Kernels export), bo
 ctypes-backed ops of kernels/_ops.py.
 
 Beside the nine stand the operators of serving from a paged K / V cache, which the reference does not have:
-kv_append and paged_attention.
+kv_append, paged_attention and sample.
 """
 from __future__ import annotations
 
@@ -15,11 +15,11 @@ from . import _ops, host
 host.bind(_ops)
 
 from . import (cross_entropy, flash_attention, fused_mlp, kv_append, layernorm, matmul,  # noqa: E402
-               paged_attention, reduce, rmsnorm, rotary_embedding, softmax)
+               paged_attention, reduce, rmsnorm, rotary_embedding, sample, softmax)
 
 MODULES = {m.KERNEL_TYPE: m for m in (matmul, softmax, layernorm, rmsnorm, flash_attention,
                                       fused_mlp, cross_entropy, rotary_embedding, reduce,
-                                      kv_append, paged_attention)}
+                                      kv_append, paged_attention, sample)}
 KERNELS = {name: m.kernel_fn for name, m in MODULES.items()}
 
 

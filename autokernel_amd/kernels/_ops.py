@@ -285,3 +285,11 @@ def paged_attn(o: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache:
          q_starts.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, *sizes, _I64x2(*q.stride()[:2]),
          _I64x3(*k_cache.stride()[:3]), _I64x3(*v_cache.stride()[:3]), _I64x2(*o.stride()[:2]), float(sm_scale),
          _lib.ptr(ws), nbytes)
+
+
+def sample(tokens: torch.Tensor, logits: torch.Tensor, u: torch.Tensor, temperature, top_k, top_p, min_p) -> None:
+    """One token per row of logits [rows, vocab]; each setting a number or a [rows] tensor."""
+    def arg(v):
+        return (v.data_ptr(), 0) if torch.is_tensor(v) else (None, v)
+    _run("ak_sample", logits, None, _code(logits, "sample"), logits.data_ptr(), u.data_ptr(), tokens.data_ptr(),
+         logits.shape[0], logits.shape[1], _ld(logits), *arg(temperature), *arg(top_k), *arg(top_p), *arg(min_p))

@@ -387,6 +387,28 @@ int ak_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_c
                   const int64_t* k_cache_strides, const int64_t* v_cache_strides, const int64_t* o_strides,
                   float sm_scale, void* workspace, int64_t workspace_bytes, hipStream_t stream);
 
+/*
+ * One token per row of logits [rows, vocab] (row_stride elements apart) from one random number each. With
+ * x a row, M its maximum and w_i = exp((x_i - M) / temperature), in falling order of x (equal values: lowest
+ * index first), each step on what the one before has left:
+ *   min-p: w_i >= min_p (min_p <= 0: all; above 1: as 1)
+ *   top-k: the first top_k (top_k <= 0: all)
+ *   top-p: the shortest prefix whose mass reaches top_p of theirs, one element at least (top_p >= 1: all)
+ *   the token: the first element whose running mass exceeds u times the mass kept
+ * temperature 0 takes the maximum (lowest index). u: fp32 [rows], taken as 0 below 0 and as 1 - 2^-24 above
+ * it. Each setting is a scalar, or an array with one value per row where its _rows pointer is not NULL.
+ * tokens: int64 [rows]; -1 for a row that holds a NaN, one whose maximum is -infinity and one with a setting
+ * from an array that is a NaN or, for the temperature, negative or infinite (as scalars: AK_EINVAL).
+ * +infinity takes all the weight (shared by all of them). Weights and their sums are exact to better than 2^-40
+ * and independent of any order, so a row and its number always give the same token. vocab up to 2^20
+ * (above: AK_EUNSUPPORTED).
+ * No counterpart in the reference, whose models end at their logits (models/llama_7b.py:160-171).
+ */
+int ak_sample(int dtype, const void* logits, const float* u, int64_t* tokens, int64_t rows, int64_t vocab,
+              int64_t row_stride, const float* temperature_rows, float temperature, const int32_t* top_k_rows,
+              int32_t top_k, const float* top_p_rows, float top_p, const float* min_p_rows, float min_p,
+              hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -108,3 +108,20 @@ def test_pages_of_positions_on_the_host(tmp_path):
                    capture_output=True, timeout=300)
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+def test_sample_refusals(lib):
+    from autokernel_amd import _lib
+    x = ctypes.c_void_p(4096)
+    base = dict(dtype=1, x=x, u=x, out=x, rows=4, vocab=100, stride=100, tp=None, t=1.0, kp=None, k=0, pp=None, p=1.0,
+                mp=None, m=0.0, stream=None)
+
+    def call(**kw):
+        return lib.ak_sample(*{**base, **kw}.values())
+    nan = float("nan")
+    for bad in (dict(dtype=7), dict(rows=-1), dict(vocab=0), dict(vocab=-5), dict(stride=99), dict(stride=-1), dict(x=None),
+                dict(u=None), dict(out=None), dict(t=-1.0), dict(t=nan), dict(t=float("inf")), dict(p=nan), dict(m=nan),
+                dict(rows=1 << 31), dict(rows=1 << 30)):
+        assert call(**bad) == _lib.AK_EINVAL, bad
+    assert call(vocab=(1 << 20) + 1, stride=1 << 21) == _lib.AK_EUNSUPPORTED
+    assert call(rows=0) == _lib.AK_OK
