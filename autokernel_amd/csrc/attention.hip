@@ -28,12 +28,6 @@
 
 namespace ak {
 
-constexpr int kFaBKV = 64;   // keys per tile
-// fa_fwd2's lazy exp2 base: a row's base is raised only when a tile's max passes it by more than
-// this (log2 units), so P <= 2^8 (exact range in f16 / bf16) and, after a row's first tile, the
-// O rescale is almost never needed.
-constexpr float kFa2Slack = 8.0f;
-
 constexpr int kFaWaves = 4;                  // waves per block, 32 query rows each
 constexpr int kFaBQ = 32 * kFaWaves;         // query rows per block
 constexpr int kFaThreads = kFaWaves * 64;
@@ -45,17 +39,6 @@ __device__ __forceinline__ int fa_swz(int row, int c) { return c ^ (row & 7); }
 // Physical position of key offset o (0..15) inside its 16-key group in V^T: the MFMA's logical
 // k index h*8 + e (lane half h, element e) carries key 4h + (e & 3) + 8 * (e >> 2).
 __device__ __forceinline__ int fa_kperm(int o) { return o ^ ((((o >> 2) ^ (o >> 3)) & 1) * 12); }
-
-template <typename T>
-__device__ __forceinline__ f32x16 mfma32x32x16(const u32x4& a, const u32x4& b, const f32x16& c);
-template <>
-__device__ __forceinline__ f32x16 mfma32x32x16<TF16>(const u32x4& a, const u32x4& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f32x16 mfma32x32x16<TBF16>(const u32x4& a, const u32x4& b, const f32x16& c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
 
 template <typename T, int D>
 __global__ __launch_bounds__(kFaThreads, 8 / kFaWaves) void fa_fwd(
@@ -333,59 +316,6 @@ __global__ __launch_bounds__(kFaThreads, 8 / kFaWaves) void fa_fwd(
 //      (groups 0, 1) or r+4..r+7 (groups 2, 3) at 32 bytes each; any two of its groups land on
 //      distinct banks.
 // ============================================================================================
-template <int D>
-__device__ __forceinline__ int fa2_kswz(int r) {
-  if constexpr (D == 128) return r & 15;
-  else return (r >> 1) & 7;
-}
-template <int D>
-__device__ __forceinline__ int fa2_vswz(int r) {
-  if constexpr (D == 128) return 4 * (r & 3) + 2 * ((r >> 2) & 1);
-  else return 4 * ((r >> 1) & 1) + 2 * ((r >> 2) & 1);
-}
-
-// Raw buffer resource: loads at byte offsets >= nbytes return zeros.
-__device__ __forceinline__ u32x4 fa2_rsrc(const void* base, uint32_t nbytes) {
-  const uint64_t a = (uint64_t)(uintptr_t)base;
-  u32x4 r;
-  r[0] = __builtin_amdgcn_readfirstlane((uint32_t)a);
-  r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);  // stride 0
-  r[2] = __builtin_amdgcn_readfirstlane(nbytes);
-  r[3] = 0x00020000u;  // 32-bit data format, untyped access
-  return r;
-}
-
-// One 1 KB LDS-DMA transfer: lane L's 16 bytes from rsrc + voff land at LDS byte lds + 16 L.
-// Inline assembly, so the compiler inserts no waits for it: every wait is an explicit vmcnt. The
-// LDS destination is an input operand bound to M0 ("{m0}"): the compiler writes M0 itself, so no
-// register changes behind its back. One wait state separates the M0 write from the load.
-__device__ __forceinline__ void fa2_dma16(const u32x4& rsrc, uint32_t voff, uint32_t lds) {
-  asm volatile(
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %0, %1, 0 offen lds"
-      :
-      : "v"(voff), "s"(rsrc), "{m0}"(lds)
-      : "memory");
-}
-
-typedef short fa2_s16x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ u32x2 fa2_tr16(const uint16_t* p) {
-  return __builtin_bit_cast(
-      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) fa2_s16x4*)(p)));
-}
-
-// Keeps the computation of x ahead of this point (an empty use the compiler cannot move).
-__device__ __forceinline__ void fa2_pin(const f32x16& x) { asm volatile("" ::"v"(x)); }
-// max over the two 32-lane halves (every lane gets the same value, combined in the same order)
-__device__ __forceinline__ float fa2_halves_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fa2_max(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float fa2_halves_sum(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // fa_fwd2 work split: kFa2Waves waves of 32 query rows per block, two waves per SIMD.
 constexpr int kFa2Waves = 4;
 constexpr int kFa2BQ = 32 * kFa2Waves;

@@ -7,9 +7,10 @@
 // its page table.
 //
 // Work split. The rows of a (sequence, KV head) are its group's query heads of each new token, token by
-// token (row r: token r / group, head r % group), cut into tiles. A tile's keys are cut into slices of C
+// token (row r: token r / group, head r % group), cut into tiles: of 128 rows for sequences of more than
+// kPaSplitRows of them (pa_tiles), of 16 for the others (pa_rows). A tile's keys are cut into slices of C
 // keys, and a block takes one (tile, slice). The lengths are device data, so every block finds its item
-// itself: it adds up the batch's work, derives C (about `target` items in all) and walks the sequences'
+// itself: it adds up its class's work, derives C (about `target` items in all) and walks the sequences'
 // item counts. The grid covers the most items there can be; blocks past the last one end at once. Sliced
 // rows leave fp32 partials (max, sum, weighted values) that pa_merge combines in slice order, so results
 // do not depend on the order in which blocks run.
@@ -26,16 +27,21 @@ namespace ak {
 constexpr int kPaWaves = 4;
 constexpr int kPaThreads = kPaWaves * kWave;
 
+// Sequences with few rows, or with many: their tiles of BM rows.
+struct PaClass {
+  float *part, *stat;  // [items][BM][Dp], [items][BM][2] (exp2 base, sum)
+  float target;        // items aimed at; 0: keys are not sliced
+  uint32_t items;      // the most items there can be
+};
 struct PaArgs {
   const void *q, *kc, *vc;
   void* o;
-  float *part, *stat;  // [items][tile rows][Dp], [items][tile rows][2] (exp2 base, sum)
+  PaClass c[2];    // few rows, many rows
+  int split_rows;  // most rows (new tokens times group) of a sequence of class 0
   int64_t qst, qsh, ost, osh;            // row and head strides (elements)
   int64_t kcp, kch, kct, vcp, vch, vct;  // cache: page, head, slot strides
   int Hq, Hk, G, D, Dp, vec;  // Dp: floats of a partial row, D rounded up to 4
   float c_log2;
-  float target;    // items aimed at; 0: keys are not sliced
-  uint32_t items;  // grid of the attention kernel: the most items there can be
   FastDiv f_g, f_hk;
   PagedSeqs s;
 };
@@ -55,8 +61,8 @@ __device__ __forceinline__ PaSeq pa_seq(const PagedSeqs& s, int b) {
 }
 
 struct PaItem {
-  int b, hk, tile, split, nsplit, chunk, tiles;
-  uint32_t first;  // index of the sequence's first item
+  int b, hk, tile, split, nsplit, chunk;
+  uint32_t slot;  // the item's place among its class's partials
   PaSeq seq;
 };
 
@@ -69,40 +75,46 @@ __device__ __forceinline__ int pa_wave_scan(int v) {  // inclusive
   return v;
 }
 
-// Keys per slice: all of them when the batch's work fills the chip without slicing, else the work over
+// Keys per slice: all of them when the class's work fills the chip without slicing, else the work over
 // `target`, in multiples of kPaSlice.
 constexpr int kPaSlice = 256;
-template <int BM>
+template <int BM, int CLS>
+__device__ __forceinline__ int pa_tiles_of(const PaArgs& a, const PaSeq& q) {
+  const int rows = q.n * a.G;
+  return (CLS == 0) == (rows <= a.split_rows) ? (rows + BM - 1) / BM : 0;
+}
+template <int BM, int CLS>
 __device__ __forceinline__ int pa_chunk(const PaArgs& a) {
-  if (a.target <= 0.f) return INT_MAX;
+  if (a.c[CLS].target <= 0.f) return INT_MAX;
   float w = 0.f;
   for (int i = 0; i < a.s.B; i += kWave) {
     const int b = i + lane_id();
     if (b >= a.s.B) break;
     const PaSeq q = pa_seq(a.s, b);
-    w += (float)((q.n * a.G + BM - 1) / BM) * (float)q.len;
+    w += (float)pa_tiles_of<BM, CLS>(a, q) * (float)q.len;
   }
   w = wave_sum(w) * (float)a.Hk * 1.001f;
-  const float c = ceilf(w / a.target / (float)kPaSlice) * (float)kPaSlice;
+  const float c = ceilf(w / a.c[CLS].target / (float)kPaSlice) * (float)kPaSlice;
   return c >= 1e9f ? INT_MAX : max((int)c, kPaSlice);
 }
 __device__ __forceinline__ int pa_splits(int len, int chunk) {
   return chunk == INT_MAX ? 1 : max(1, (len + chunk - 1) / chunk);
 }
 
-// Item `it` of the batch; false when there are fewer. Within a sequence the KV heads run fastest (one
+// Item `it` of a class; false when there are fewer. Within a sequence the KV heads run fastest (one
 // per XCD, whose L2 then serves the tiles that share a head's keys), then tiles, last rows first (they see
 // the most keys), then slices.
-template <int BM>
+template <int BM, int CLS>
 __device__ __forceinline__ bool pa_find(const PaArgs& a, uint32_t it, PaItem& o) {
-  o.chunk = pa_chunk<BM>(a);
+  o.chunk = pa_chunk<BM, CLS>(a);
+  o.slot = it;
   uint32_t base = 0;
   for (int i = 0; i < a.s.B; i += kWave) {
     const int b = i + lane_id();
     int cnt = 0, tiles = 0;
     if (b < a.s.B) {
       const PaSeq q = pa_seq(a.s, b);
-      tiles = (q.n * a.G + BM - 1) / BM;
+      tiles = pa_tiles_of<BM, CLS>(a, q);
       cnt = tiles * a.Hk * pa_splits(q.len, o.chunk);
     }
     const int inc = pa_wave_scan(cnt);
@@ -110,15 +122,18 @@ __device__ __forceinline__ bool pa_find(const PaArgs& a, uint32_t it, PaItem& o)
     if (hit) {
       const int l = __builtin_ctzll(hit);
       o.b = i + l;
-      o.tiles = __builtin_amdgcn_readlane(tiles, l);
-      o.first = base + (uint32_t)__builtin_amdgcn_readlane(inc - cnt, l);
+      tiles = __builtin_amdgcn_readlane(tiles, l);
       o.seq = pa_seq(a.s, o.b);
+      o.seq.t0 = __builtin_amdgcn_readfirstlane(o.seq.t0);  // one sequence: keep it in scalar registers
+      o.seq.n = __builtin_amdgcn_readfirstlane(o.seq.n);
+      o.seq.len = __builtin_amdgcn_readfirstlane(o.seq.len);
+      o.chunk = __builtin_amdgcn_readfirstlane(o.chunk);
       o.nsplit = pa_splits(o.seq.len, o.chunk);
-      const uint32_t rel = it - o.first;
+      const uint32_t rel = it - base - (uint32_t)__builtin_amdgcn_readlane(inc - cnt, l);
       const uint32_t x = fdiv(rel, a.f_hk);
       o.hk = (int)(rel - x * a.Hk);
-      o.split = (int)(x / (uint32_t)o.tiles);
-      o.tile = o.tiles - 1 - (int)(x - (uint32_t)o.split * o.tiles);
+      o.split = (int)(x / (uint32_t)tiles);
+      o.tile = tiles - 1 - (int)(x - (uint32_t)o.split * tiles);
       return o.split < o.nsplit;
     }
     base += (uint32_t)__builtin_amdgcn_readlane(inc, kWave - 1);
@@ -208,10 +223,10 @@ __device__ __forceinline__ float pa_inv(const PaSeq& q, bool sees, float l) {
   return q.overlong ? __builtin_nanf("") : sees ? 1.0f / l : 0.f;
 }
 
-// Rows r_begin .. r_end - 1 of an item's tile (of `bm` rows) over keys [lo, hi), one wave per row: results, or
-// partials when the keys are sliced.
-template <typename T>
-__device__ void pa_rows_again(const PaArgs& a, const PaItem& it, int r_begin, int r_end, int lo, int hi, int bm) {
+// Rows r_begin .. r_end - 1 of an item's tile over keys [lo, hi), one wave per row: results, or partials when
+// the keys are sliced.
+template <typename T, int BM, int CLS>
+__device__ void pa_one_by_one(const PaArgs& a, const PaItem& it, int r_begin, int r_end, int lo, int hi) {
   using S = typename T::S;
   const int lane = lane_id();
   for (int r = r_begin + wave_id(); r < r_end; r += kPaWaves) {
@@ -221,14 +236,14 @@ __device__ void pa_rows_again(const PaArgs& a, const PaItem& it, int r_begin, in
     float m, l, acc[4];
     pa_row<T>(a, it.b, it.hk, (const S*)a.q + tok * a.qst + h * a.qsh, lo, min(seen, hi), m, l, acc);
     if (it.nsplit > 1) {
-      const int64_t slot = (int64_t)blockIdx.x * bm + (r - r_begin);
-      float* p = a.part + slot * a.Dp;
+      const int64_t slot = (int64_t)it.slot * BM + (r - r_begin);
+      float* p = a.c[CLS].part + slot * a.Dp;
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         if (lane + 64 * x < a.D) p[lane + 64 * x] = acc[x];
       if (lane == 0) {
-        a.stat[slot * 2] = m;
-        a.stat[slot * 2 + 1] = l;
+        a.c[CLS].stat[slot * 2] = m;
+        a.c[CLS].stat[slot * 2 + 1] = l;
       }
       continue;
     }
@@ -245,16 +260,16 @@ constexpr int kPaRowTile = kPaWaves;
 template <typename T>
 __global__ __launch_bounds__(kPaThreads) void pa_general(const PaArgs a) {
   PaItem it;
-  if (!pa_find<kPaRowTile>(a, blockIdx.x, it)) return;
+  if (!pa_find<kPaRowTile, 0>(a, blockIdx.x, it)) return;
   const int r0 = it.tile * kPaRowTile, lo = it.nsplit == 1 ? 0 : it.split * it.chunk;
-  pa_rows_again<T>(a, it, r0, min(it.seq.n * a.G, r0 + kPaRowTile), lo, it.nsplit == 1 ? INT_MAX : lo + it.chunk,
-                   kPaRowTile);
+  pa_one_by_one<T, kPaRowTile, 0>(a, it, r0, min(it.seq.n * a.G, r0 + kPaRowTile), lo,
+                                  it.nsplit == 1 ? INT_MAX : lo + it.chunk);
 }
 
 // Sliced rows: W waves per (row, query head). A group of 16 lanes adds the partials of slices g, g + 4 W, ..
 // (lane c: dims 4 c .. 4 c + 3 of each 64), then the groups' sums combine in group order. Four groups of one
 // wave for many rows; with few rows sixteen, so that 64 slices' partials are in flight at once.
-template <typename T, int BM, int W>
+template <typename T, int BM0, int BM1, int W>
 __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
   using S = typename T::S;
   constexpr int NG = 4 * W, NR = kPaWaves / W;  // groups of a row, rows of a block
@@ -270,10 +285,12 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
   if (b < a.s.B) {
     q = pa_seq(a.s, b);
     if (tok >= q.t0 && tok < q.t0 + q.n) {
-      chunk = pa_chunk<BM>(a);
+      chunk = q.n * a.G <= a.split_rows ? pa_chunk<BM0, 0>(a) : pa_chunk<BM1, 1>(a);
       nsplit = pa_splits(q.len, chunk);
     }
   }
+  const int cls = q.n * a.G <= a.split_rows ? 0 : 1, bm = cls ? BM1 : BM0;
+  const PaClass& cl = a.c[cls];
   float m = -INFINITY, l = 0.f, acc[4][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
@@ -284,12 +301,12 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
     int first = 0;
     for (int i = lane; i < b; i += kWave) {
       const PaSeq x = pa_seq(a.s, i);
-      first += (x.n * a.G + BM - 1) / BM * a.Hk * pa_splits(x.len, chunk);
+      first += (cls ? pa_tiles_of<BM1, 1>(a, x) : pa_tiles_of<BM0, 0>(a, x)) * a.Hk * pa_splits(x.len, chunk);
     }
     first = __builtin_amdgcn_readlane(pa_wave_scan(first), kWave - 1);
-    const int tiles = (q.n * a.G + BM - 1) / BM;
+    const int tiles = (q.n * a.G + bm - 1) / bm;
     const int hk = h / a.G, r = ((int)tok - q.t0) * a.G + h % a.G;
-    const uint32_t it0 = (uint32_t)first + (uint32_t)(tiles - 1 - r / BM) * a.Hk + hk;
+    const uint32_t it0 = (uint32_t)first + (uint32_t)(tiles - 1 - r / bm) * a.Hk + hk;
     for (int sp = g; sp < nsplit; sp += 4 * NG) {
       float ms[4], ls[4];
       f32x4 v[4][4];
@@ -298,13 +315,13 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
         const uint32_t it = it0 + (uint32_t)(sp + u * NG) * tiles * a.Hk;
         ms[u] = -INFINITY;
         ls[u] = 0.f;
-        if (sp + u * NG >= nsplit || it >= a.items) continue;
-        const int64_t slot = (int64_t)it * BM + r % BM;
-        ms[u] = a.stat[slot * 2];
-        ls[u] = a.stat[slot * 2 + 1];
+        if (sp + u * NG >= nsplit || it >= cl.items) continue;
+        const int64_t slot = (int64_t)it * bm + r % bm;
+        ms[u] = cl.stat[slot * 2];
+        ls[u] = cl.stat[slot * 2 + 1];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (64 * j + 4 * c < a.D) v[u][j] = *reinterpret_cast<const f32x4*>(a.part + slot * a.Dp + 64 * j + 4 * c);
+          if (64 * j + 4 * c < a.D) v[u][j] = *reinterpret_cast<const f32x4*>(cl.part + slot * a.Dp + 64 * j + 4 * c);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -382,18 +399,20 @@ struct PrVec<64> {
   typedef u32x2 type;
 };
 
+template <int D>
+struct PrShared {
+  float so[kPaWaves][kPrRows][D + 4];
+  float st[kPaWaves][kPrRows][2];
+  int again;
+};
 template <typename T, int D, int PG>
-__global__ __launch_bounds__(kPaThreads, 2) void pa_rows(const PaArgs a) {
+__device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrShared<D>& sh) {
   constexpr int NS = D / 32, VW = D / 16;
   constexpr int NK = PG == 8 ? 1 : 2, NV = PG == 8 ? 1 : 8;  // page numbers of a lane and step
   using VV = typename PrVec<D>::type;
-  __shared__ __attribute__((aligned(16))) float so[kPaWaves][kPrRows][D + 4];
-  __shared__ float sst[kPaWaves][kPrRows][2];
-  __shared__ int again;
-
   PaItem it;
-  if (!pa_find<kPrRows>(a, blockIdx.x, it)) return;
-  if (threadIdx.x == 0) again = 0;
+  if (!pa_find<kPrRows, 0>(a, item, it)) return;
+  if (threadIdx.x == 0) sh.again = 0;
   const int lane = lane_id(), w = wave_id();
   const int i16 = lane & 15, g = lane >> 4;
   const uint16_t* Kb = (const uint16_t*)a.kc + it.hk * a.kch + g * 8;
@@ -545,40 +564,40 @@ __global__ __launch_bounds__(kPaThreads, 2) void pa_rows(const PaArgs a) {
 #pragma unroll
   for (int v = 0; v < 4; ++v)
 #pragma unroll
-    for (int e = 0; e < VW; ++e) so[w][i16][VW * (4 * g + v) + e] = o[e][v];
+    for (int e = 0; e < VW; ++e) sh.so[w][i16][VW * (4 * g + v) + e] = o[e][v];
   if (g == 0) {
-    sst[w][i16][0] = m_run;
-    sst[w][i16][1] = l_run;
+    sh.st[w][i16][0] = m_run;
+    sh.st[w][i16][1] = l_run;
   }
   __syncthreads();  // (the flag is cleared by now)
-  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) atomicOr(&again, 1);
+  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) atomicOr(&sh.again, 1);
   __syncthreads();
-  if (again) {
-    pa_rows_again<T>(a, it, r0, min(rows, r0 + kPrRows), kbeg, kend, kPrRows);
+  if (sh.again) {
+    pa_one_by_one<T, kPrRows, 0>(a, it, r0, min(rows, r0 + kPrRows), kbeg, kend);
     return;
   }
   const int q = threadIdx.x >> 4, c = threadIdx.x & 15;  // row of the tile, VW dims at c * VW
   if (r0 + q >= rows) return;
   float mb = -INFINITY, l = 0.f, acc[VW];
 #pragma unroll
-  for (int x = 0; x < kPaWaves; ++x) mb = fmaxf(mb, sst[x][q][0]);
+  for (int x = 0; x < kPaWaves; ++x) mb = fmaxf(mb, sh.st[x][q][0]);
 #pragma unroll
   for (int e = 0; e < VW; ++e) acc[e] = 0.f;
 #pragma unroll
   for (int x = 0; x < kPaWaves; ++x) {
-    const float f = sst[x][q][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sst[x][q][0] - mb);
-    l += sst[x][q][1] * f;
+    const float f = sh.st[x][q][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh.st[x][q][0] - mb);
+    l += sh.st[x][q][1] * f;
 #pragma unroll
-    for (int e = 0; e < VW; ++e) acc[e] += so[x][q][c * VW + e] * f;
+    for (int e = 0; e < VW; ++e) acc[e] += sh.so[x][q][c * VW + e] * f;
   }
   if (it.nsplit > 1) {
-    const int64_t slot = (int64_t)blockIdx.x * kPrRows + q;
-    float* p = a.part + slot * a.Dp + c * VW;
+    const int64_t slot = (int64_t)it.slot * kPrRows + q;
+    float* p = a.c[0].part + slot * a.Dp + c * VW;
 #pragma unroll
     for (int e = 0; e < VW; e += 4) *reinterpret_cast<f32x4*>(p + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
     if (c == 0) {
-      a.stat[slot * 2] = mb;
-      a.stat[slot * 2 + 1] = l;
+      a.c[0].stat[slot * 2] = mb;
+      a.c[0].stat[slot * 2 + 1] = l;
     }
     return;
   }
@@ -591,65 +610,478 @@ __global__ __launch_bounds__(kPaThreads, 2) void pa_rows(const PaArgs a) {
                          (int64_t)(it.hk * a.G + r0 + q - tk * a.G) * a.osh + c * VW) = pk;
 }
 
-// Most items a call can have, and its workspace. Keys are sliced only where some sequence can be longer
-// than one slice.
-struct PaPlan {
-  int64_t items, ws_bytes;
-  float target;
+// Many rows per KV head: 128 rows a block, a wave owns 32, 64 keys a step through LDS. The pipeline of fa_fwd2
+// (attention.hip: S^T = K Q^T and O^T += V^T P^T on v_mfma_f32_32x32x16, K and V by LDS DMA two stages deep, V
+// read transposed by ds_read_b64_tr_b16, each MFMA burst beside the other product's softmax work, the
+// lazily raised exp2 base). What is different:
+//   * A row is a (token, head of the group) pair, so the query heads of a KV head share its K and V tiles.
+//   * A DMA transfer covers 4 (head_dim 128) or 8 (64) keys and so, with pages of a multiple of 8 slots, lies
+//     in one page: a wave makes each transfer's buffer resource from that page's address, with as many
+//     bytes as the page has keys of the slice left (the rest arrives as zeros). The slice's page numbers wait in
+//     LDS (a ring of kPtWin, refilled by halves), read one tile ahead.
+//   * No pass over what a row does not see: V of masked keys only has to be finite. Where a row's result is
+//     NaN, or a page lies outside the cache, the item's rows are computed again by pa_row.
+// Bound by the MFMA and the softmax VALU work, as fa_fwd2 is.
+constexpr int kPtRows = 32 * kPaWaves, kPtWin = 2048;
+
+// fa2_dma16 for a resource made right before it: its words come from v_readlane / v_readfirstlane, and a vector
+// memory instruction may read a scalar register that the VALU wrote only five wait states later. The compiler
+// keeps that distance for its own instructions but does not see the load in here.
+__device__ __forceinline__ void pa_dma16(const u32x4& rsrc, uint32_t voff, uint32_t lds) {
+  asm volatile(
+      "s_nop 4\n\t"
+      "buffer_load_dwordx4 %0, %1, 0 offen lds"
+      :
+      : "v"(voff), "s"(rsrc), "{m0}"(lds)
+      : "memory");
+}
+template <int D>
+struct PtShared {
+  uint16_t k[2 * kFaBKV * D], v[2 * kFaBKV * D];
+  int page[kPtWin];
+  int again;
 };
-static PaPlan pa_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t keys, int bm, int64_t target) {
-  PaPlan p;
-  const int64_t tiles = (T * (Hq / Hk)) / bm + std::min(B, T);
-  p.items = tiles * Hk;
-  p.target = 0.f;
-  p.ws_bytes = 0;
-  if (keys > kPaSlice) {
-    p.items += target;
-    p.target = (float)target;
-    p.ws_bytes = p.items * bm * ((D + 3) / 4 * 4 + 2) * (int64_t)sizeof(float);
+template <typename T, int D>
+__device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, PtShared<D>& sh) {
+  constexpr int DC = D / 8;                            // 16-byte chunks per key
+  constexpr int RPI = 64 / DC;                         // keys per 1 KB transfer
+  constexpr int NIW = kFaBKV / RPI / kPaWaves;         // transfers per wave and tile, per matrix
+  constexpr int NS = D / 16, NDB = D / 32;             // 16-deep steps of S^T, 32-row blocks of O^T
+  constexpr int TILE = kFaBKV * D;
+  PaItem it;
+  if (!pa_find<kPtRows, 1>(a, item, it)) return;
+  if (threadIdx.x == 0) sh.again = 0;
+  const int lane = lane_id(), l32 = lane & 31, hh = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(wave_id());
+  const int rows = it.seq.n * a.G, r0 = it.tile * kPtRows, rw0 = r0 + 32 * w;  // this wave's first row
+  const int my_r = rw0 + l32;
+  const int kbeg = it.nsplit == 1 ? 0 : it.split * it.chunk;
+  const int kend = min(pa_seen(it, min(rows, r0 + kPtRows) - 1, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk);
+  const int tk = (int)fdiv((uint32_t)min(my_r, rows - 1), a.f_g);
+  const int64_t head = it.hk * a.G + min(my_r, rows - 1) - tk * a.G, tok = it.seq.t0 + tk;
+  const int nt = (max(kend - kbeg, 0) + kFaBKV - 1) / kFaBKV;
+  float m_run = -INFINITY, l_run = 0.f;
+  f32x16 o[NDB];
+#pragma unroll
+  for (int i = 0; i < NDB; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[i][v] = 0.f;
+  bool bad = false;
+
+  if (nt > 0) {
+    // keys seen by this lane's row, by the wave's first row and by its last
+    const int lim = min(pa_seen(it, min(my_r, rows - 1), a.f_g), kend);
+    const int lim0 = min(pa_seen(it, min(rw0, rows - 1), a.f_g), kend);
+    const int lim1 = min(pa_seen(it, min(rw0 + 31, rows - 1), a.f_g), kend);
+    const int jw = rw0 < rows && lim1 > kbeg ? (lim1 - 1 - kbeg) / kFaBKV : -1;  // the wave's last tile
+
+    // page numbers kbeg / page_size .. (kend - 1) / page_size, entry e at e % kPtWin
+    const int32_t* tab = a.s.table + it.b * a.s.table_stride;
+    const int e_last = (int)fdiv((uint32_t)(kend - 1), a.s.page_div);
+    constexpr int kHalf = kPtWin / 2;
+    int half = (int)fdiv((uint32_t)kbeg, a.s.page_div) / kHalf;  // the half that V's transfers have come to
+    auto fill = [&](int h) {
+      for (int e = h * kHalf + (int)threadIdx.x; e < (h + 1) * kHalf && e <= e_last; e += kPaThreads)
+        sh.page[e % kPtWin] = tab[e];
+    };
+    fill(half);
+    fill(half + 1);
+    __syncthreads();
+    auto page_of = [&](int j) {  // lane i % NIW: page number of transfer i of tile j
+      const int key = min(kbeg + j * kFaBKV + ((lane & (NIW - 1)) * kPaWaves + w) * RPI, kend - 1);
+      return sh.page[fdiv((uint32_t)key, a.s.page_div) % kPtWin];
+    };
+
+    const uint16_t* Qr = (const uint16_t*)a.q + tok * a.qst + head * a.qsh;
+    u32x4 qf[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = my_r < rows ? ld16(Qr + s * 16 + hh * 8) : u32x4{0u, 0u, 0u, 0u};
+
+    // Byte offsets of a lane inside a transfer: lane L writes physical chunk L % DC of row L / DC and so
+    // fetches the logical chunk that the swizzle maps there.
+    uint32_t offk[NIW], offv[NIW];
+#pragma unroll
+    for (int i = 0; i < NIW; ++i) {
+      const int row = (i * kPaWaves + w) * RPI + lane / DC, pc = lane % DC;
+      offk[i] = (uint32_t)((lane / DC) * (int)a.kct * 2 + ((pc ^ fa2_kswz<D>(row)) * 16));
+      offv[i] = (uint32_t)((lane / DC) * (int)a.vct * 2 + ((pc ^ fa2_vswz<D>(row)) * 16));
+    }
+    const uint32_t sK_lds = (uint32_t)(uintptr_t)(lds_void*)sh.k, sV_lds = (uint32_t)(uintptr_t)(lds_void*)sh.v;
+    auto issue = [&](const uint16_t* base, int64_t ps, int64_t ss, const uint32_t (&off)[NIW], int pages, int j,
+                     uint32_t lds) {
+#pragma unroll
+      for (int i = 0; i < NIW; ++i) {
+        const int key = kbeg + j * kFaBKV + (i * kPaWaves + w) * RPI;
+        const int left = min(kend - key, RPI);
+        const int pg = __builtin_amdgcn_readlane(pages, i);
+        const int slot = key - (int)fdiv((uint32_t)key, a.s.page_div) * a.s.page_size;
+        const bool in = (uint32_t)pg < a.s.num_pages;
+        bad |= !in && left > 0;
+        const u32x4 rs = fa2_rsrc(in ? base + pg * ps + slot * ss : base,
+                                  in && left > 0 ? (uint32_t)(((left - 1) * (int)ss + D) * 2) : 0u);
+        pa_dma16(rs, off[i], lds + (i * kPaWaves + w) * 1024);
+      }
+    };
+    const uint16_t* Kb = (const uint16_t*)a.kc + it.hk * a.kch;
+    const uint16_t* Vb = (const uint16_t*)a.vc + it.hk * a.vch;
+    int pk = page_of(0), pv_ = pk;  // page numbers of the next K and V tile to be issued
+    auto issue_k = [&](int j, int stage) {
+      issue(Kb, a.kcp, a.kct, offk, pk, j, sK_lds + stage * TILE * 2);
+      pk = page_of(j + 1);
+    };
+    auto issue_v = [&](int j, int stage) {
+      issue(Vb, a.vcp, a.vct, offv, pv_, j, sV_lds + stage * TILE * 2);
+      const int h = (int)fdiv((uint32_t)(kbeg + j * kFaBKV), a.s.page_div) / kHalf;
+      // every wave's V numbers of this half's tiles on come from this half or the next, every K number read so
+      // far too: the half behind can take the one after
+      if (h > half) {
+        half = h;
+        fill(half + 1);
+      }
+      pv_ = page_of(j + 1);
+    };
+
+    auto qk = [&](const uint16_t* ks, f32x16 (&s)[2]) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[kb][v] = 0.f;
+#pragma unroll
+      for (int st = 0; st < NS; ++st)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+          const int r = kb * 32 + l32, c = st * 2 + hh;
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(&ks[r * D + (c ^ fa2_kswz<D>(r)) * 8]);
+          s[kb] = mfma32x32x16<T>(kf, qf[st], s[kb]);
+        }
+    };
+    const int g16 = lane >> 4, i16 = lane & 15;
+    const int vrow = 4 * (g16 >> 1) + (i16 >> 2), vcol = 16 * (g16 & 1) + 4 * (i16 & 3), vsw = fa2_vswz<D>(vrow);
+    u32x4 pf[4];
+    auto pv = [&](const uint16_t* vs) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int col = db * 32 + vcol;
+          const uint16_t* p = vs + (16 * t + vrow) * D + (((col >> 3) ^ vsw) * 8) + (col & 7);
+          const u32x2 lo = fa2_tr16(p), hi = fa2_tr16(p + 8 * D);
+          o[db] = mfma32x32x16<T>(u32x4{lo[0], lo[1], hi[0], hi[1]}, pf[t], o[db]);
+        }
+    };
+    // Row statistics of S_j: mask, tile max, lazy base update (alpha = 1 unless it moved).
+    auto stats = [&](f32x16 (&s)[2], int k0, bool masked, float& alpha, float& base) {
+      if (masked) {
+        const int t = lim - (k0 + hh * 4);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int off = kb * 32 + (v >> 2) * 8 + (v & 3);
+            if (off >= t) s[kb][v] = -INFINITY;
+          }
+      }
+      float m4[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int kb = c >> 1, v0 = (c & 1) * 8;
+        float m = fa2_max(fa2_max(s[kb][v0], s[kb][v0 + 1]), s[kb][v0 + 2]);
+        m = fa2_max(fa2_max(m, s[kb][v0 + 3]), s[kb][v0 + 4]);
+        m4[c] = fa2_max(fa2_max(m, s[kb][v0 + 5]), s[kb][v0 + 6]);
+      }
+      float mt = fa2_max(fa2_max(m4[0], s[0][7]), m4[1]);
+      mt = fa2_max(fa2_max(mt, s[0][15]), m4[2]);
+      mt = fa2_max(fa2_max(mt, s[1][7]), m4[3]);
+      mt = fa2_max(mt, s[1][15]);
+      const float mts = fa2_halves_max(mt) * a.c_log2;
+      const float m_new = (mts > m_run + kFa2Slack || m_run == -INFINITY) ? fmaxf(m_run, mts) : m_run;
+      base = (m_new == -INFINITY) ? 0.f : m_new;
+      alpha = (m_new == m_run) ? 1.0f : __builtin_amdgcn_exp2f(m_run - base);
+      m_run = m_new;
+    };
+    auto exp_args = [&](f32x16 (&s)[2], float base) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[kb][v] = __builtin_fmaf(s[kb][v], a.c_log2, -base);
+    };
+    auto exp_pack = [&](const f32x16 (&s)[2]) -> float {
+      float ps = 0.f;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = 8 * (t & 1) + 2 * e;
+          pf[t][e] = fa2_pack<T>(__builtin_amdgcn_exp2f(s[t >> 1][v]), __builtin_amdgcn_exp2f(s[t >> 1][v + 1]));
+          ps = fa2_sum2<T>(pf[t][e], ps);
+        }
+      return ps;
+    };
+    auto rescale = [&](float alpha) {
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+        for (int db = 0; db < NDB; ++db)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[db][v] *= alpha;
+      }
+    };
+    // The DMA schedule and its waits are fa_fwd2's: tile t lives in stage t & 1; V_{j+1} is issued after
+    // phase 1 of iteration j, K_{j+3} after phase 2, and a wait leaves the transfers issued later in flight.
+    // (page_of's LDS reads and fill's global loads come after them; the compiler's own waits cover those.)
+    auto barrier_after = [&](int later) {
+      if (later >= 2) dma_barrier<2 * NIW>();
+      else if (later == 1) dma_barrier<NIW>();
+      else dma_barrier<0>();
+    };
+    auto sync_mid = [&](int j, int par) {
+      barrier_after(j == 0 ? (nt > 2) : 1 + (j + 2 < nt));
+      if (j + 1 < nt) issue_v(j + 1, par ^ 1);
+    };
+    auto sync_end = [&](int j, int par) {
+      barrier_after((j + 2 < nt) + (j + 1 < nt));
+      if (j + 3 < nt) issue_k(j + 3, par ^ 1);
+    };
+    f32x16 sa[2], sb[2];
+    auto iter = [&](int j, int par, f32x16 (&S)[2], f32x16 (&Sn)[2]) {
+      const int k0 = kbeg + j * kFaBKV;
+      if (j > 0 && j - 1 <= jw) pv(sh.v + (par ^ 1) * TILE);  // V_{j-1}
+      float alpha = 1.0f, base = 0.f;
+      const bool act = j <= jw;
+      if (act) stats(S, k0, k0 + kFaBKV > lim0, alpha, base);
+      sync_mid(j, par);
+      if (j + 1 <= jw) qk(sh.k + (par ^ 1) * TILE, Sn);  // K_{j+1}
+      if (act) {
+        exp_args(S, base);
+        const float ps = exp_pack(S);
+        l_run = l_run * alpha + ps;
+        rescale(alpha);
+      }
+      sync_end(j, par);
+    };
+    constexpr int kPhaseMfma = D / 8, kP1Valu = D == 128 ? 4 : 8, kP2Valu = D == 128 ? 5 : 9;
+    auto iter_fast = [&](int j, int par, f32x16 (&S)[2], f32x16 (&Sn)[2]) {
+      pv(sh.v + (par ^ 1) * TILE);
+      float alpha, base;
+      stats(S, kbeg + j * kFaBKV, false, alpha, base);
+      exp_args(S, base);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) asm volatile("" ::"v"(S[kb]));
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int i = 0; i < kPhaseMfma - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, kP1Valu, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, kP1Valu, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      sync_mid(j, par);
+      qk(sh.k + (par ^ 1) * TILE, Sn);
+      const float ps = exp_pack(S);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) asm volatile("" ::"v"(pf[t]));
+      asm volatile("" ::"v"(ps));
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+#pragma unroll
+      for (int i = 0; i < kPhaseMfma - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x402, kP2Valu, 1);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+        __builtin_amdgcn_sched_group_barrier(0x402, kP2Valu, 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      rescale(alpha);
+      l_run = l_run * alpha + ps;
+      sync_end(j, par);
+    };
+
+    issue_k(0, 0);
+    if (nt > 1) issue_k(1, 1);
+    issue_v(0, 0);
+    dma_barrier<0>();
+    qk(sh.k, sa);
+    dma_barrier<0>();
+    if (nt > 2) issue_k(2, 0);
+    const int jm = max(lim0 - kbeg, 0) / kFaBKV;  // the wave's first masked tile
+    const int jf = max(1, min(jm, jw));
+    iter(0, 0, sa, sb);
+    int j = 1;
+    for (; j + 1 < jf; j += 2) {
+      iter_fast(j, 1, sb, sa);
+      iter_fast(j + 1, 0, sa, sb);
+    }
+    if (j < jf) {
+      iter_fast(j, 1, sb, sa);
+      ++j;
+    } else {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) sa[kb] = sb[kb];
+    }
+    for (; j < nt; ++j) {
+      iter(j, j & 1, sa, sb);
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) sa[kb] = sb[kb];
+    }
+    if (nt - 1 <= jw) pv(sh.v + ((nt - 1) & 1) * TILE);
+    wait_vmcnt<0>();  // no transfer outlives the block
+    l_run = fa2_halves_sum(l_run);
+    if (my_r < rows) {
+      bad |= l_run != l_run;
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) bad |= o[db][v] != o[db][v];
+    }
   }
+  __syncthreads();  // (the flag is cleared by now)
+  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) atomicOr(&sh.again, 1);
+  __syncthreads();
+  if (sh.again) {
+    pa_one_by_one<T, kPtRows, 1>(a, it, r0, min(rows, r0 + kPtRows), kbeg, kend);
+    return;
+  }
+  if (my_r >= rows) return;
+  if (it.nsplit > 1) {
+    const int64_t slot = (int64_t)it.slot * kPtRows + 32 * w + l32;
+    float* p = a.c[1].part + slot * a.Dp;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(p + db * 32 + g * 8 + hh * 4) =
+            f32x4{o[db][g * 4], o[db][g * 4 + 1], o[db][g * 4 + 2], o[db][g * 4 + 3]};
+    if (hh == 0) {
+      a.c[1].stat[slot * 2] = m_run;
+      a.c[1].stat[slot * 2 + 1] = l_run;
+    }
+    return;
+  }
+  const float inv = pa_inv(it.seq, pa_seen(it, my_r, a.f_g) > 0, l_run);
+  uint16_t* orow = (uint16_t*)a.o + tok * a.ost + head * a.osh;
+#pragma unroll
+  for (int db = 0; db < NDB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      u32x2 pk2;
+      pk2[0] = fa2_pack<T>(o[db][g * 4] * inv, o[db][g * 4 + 1] * inv);
+      pk2[1] = fa2_pack<T>(o[db][g * 4 + 2] * inv, o[db][g * 4 + 3] * inv);
+      *reinterpret_cast<u32x2*>(orow + db * 32 + g * 8 + hh * 4) = pk2;
+    }
+}
+
+template <typename T, int D, int PG>
+__global__ __launch_bounds__(kPaThreads, 2) void pa_rows(const PaArgs a) {
+  __shared__ __attribute__((aligned(16))) PrShared<D> sh;
+  pa_rows_item<T, D, PG>(a, blockIdx.x, sh);
+}
+// Both classes in one launch: the blocks of the large tiles first.
+template <typename T, int D>
+__global__ __launch_bounds__(kPaThreads, 2) void pa_mixed(const PaArgs a) {
+  __shared__ __attribute__((aligned(1024))) union {
+    PtShared<D> t;
+    PrShared<D> r;
+  } sh;
+  if (blockIdx.x < a.c[1].items) pa_tiles_item<T, D>(a, blockIdx.x, sh.t);
+  else pa_rows_item<T, D, 8>(a, blockIdx.x - a.c[1].items, sh.r);
+}
+
+// What a call launches: the most items of each class and their partials. Keys are sliced only where some
+// sequence can be longer than kPaMinSliced, below which the merge costs more than the shorter walk saves.
+constexpr int64_t kPaSplitRows = 64, kPaMinSliced = 1536;
+struct PaPlan {
+  int bm0;
+  int64_t items[2], target[2], ws[2];  // ws: floats of a class's partials
+  int64_t bytes() const { return (ws[0] + ws[1]) * (int64_t)sizeof(float); }
+};
+// fast: the MFMA kernels; paged8: pages of a multiple of 8 slots (pa_tiles)
+static PaPlan pa_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t page_size, int64_t width,
+                      bool fast) {
+  PaPlan p{};
+  const int64_t keys = page_size * width, G = Hq / Hk, rows = T * G, seqs = std::min(B, T);
+  const bool tiles = fast && page_size % 8 == 0 && rows > kPaSplitRows;
+  p.bm0 = fast ? kPrRows : kPaRowTile;
+  p.items[0] = (rows / p.bm0 + seqs) * Hk;
+  if (tiles) {
+    p.items[0] = std::min(p.items[0], seqs * (kPaSplitRows / p.bm0) * Hk);
+    p.items[1] = (rows / kPtRows + std::min(seqs, rows / (kPaSplitRows + 1))) * Hk;
+  }
+  if (keys > kPaMinSliced) {
+    p.target[0] = 1024;
+    // two tiles per CU at a time; four times that many are work enough unsliced
+    if (tiles && rows / kPtRows * Hk < 4 * 512) p.target[1] = 512;
+  }
+  const int64_t row = (D + 3) / 4 * 4 + 2;
+  for (int c = 0; c < 2; ++c)
+    if (p.target[c] > 0) {
+      p.items[c] += p.target[c];
+      p.ws[c] = p.items[c] * (c ? kPtRows : p.bm0) * row;
+    }
   return p;
 }
 
-template <typename T, int BM, typename K>
-static int pa_launch(K kernel, PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
-  a.items = (uint32_t)p.items;
-  a.target = p.target;
-  a.part = (float*)ws;
-  a.stat = a.part ? a.part + p.items * BM * a.Dp : nullptr;
-  kernel<<<dim3((unsigned)p.items), kPaThreads, 0, st>>>(a);
-  if (a.target > 0.f) {
-    const int64_t rows = (int64_t)a.s.T * a.Hq;
-    if (rows <= 4096) pa_merge<T, BM, 4><<<dim3((unsigned)rows), kPaThreads, 0, st>>>(a);
-    else pa_merge<T, BM, 1><<<dim3((unsigned)cdiv(rows, kPaWaves)), kPaThreads, 0, st>>>(a);
+static void pa_set(PaArgs& a, const PaPlan& p, void* ws) {
+  float* f = (float*)ws;
+  for (int c = 0; c < 2; ++c) {
+    a.c[c].items = (uint32_t)p.items[c];
+    a.c[c].target = (float)p.target[c];
+    a.c[c].part = f;
+    a.c[c].stat = f ? f + p.items[c] * (c ? kPtRows : p.bm0) * a.Dp : nullptr;
+    if (f) f += p.ws[c];
   }
+  a.split_rows = p.items[1] > 0 ? (int)kPaSplitRows : INT_MAX;
+}
+template <typename T, int BM0, int BM1>
+static void pa_launch_merge(const PaArgs& a, hipStream_t st) {
+  if (a.c[0].target <= 0.f && a.c[1].target <= 0.f) return;
+  const int64_t rows = (int64_t)a.s.T * a.Hq;
+  if (rows <= 4096) pa_merge<T, BM0, BM1, 4><<<dim3((unsigned)rows), kPaThreads, 0, st>>>(a);
+  else pa_merge<T, BM0, BM1, 1><<<dim3((unsigned)cdiv(rows, kPaWaves)), kPaThreads, 0, st>>>(a);
+}
+template <typename T>
+static int launch_general(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
+  pa_set(a, p, ws);
+  pa_general<T><<<dim3((unsigned)p.items[0]), kPaThreads, 0, st>>>(a);
+  pa_launch_merge<T, kPaRowTile, kPaRowTile>(a, st);
   return record_launch();
 }
 template <typename T, int D>
-static int launch_rows(const PaArgs& a, const PaPlan& p, void* ws, hipStream_t st) {
-  return a.s.page_size % 8 == 0 ? pa_launch<T, kPrRows>(pa_rows<T, D, 8>, a, p, ws, st)
-                                : pa_launch<T, kPrRows>(pa_rows<T, D, 1>, a, p, ws, st);
+static int launch_fast(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
+  pa_set(a, p, ws);
+  const dim3 grid((unsigned)(p.items[0] + p.items[1]));
+  if (p.items[1] > 0) pa_mixed<T, D><<<grid, kPaThreads, 0, st>>>(a);
+  else if (a.s.page_size % 8 == 0) pa_rows<T, D, 8><<<grid, kPaThreads, 0, st>>>(a);
+  else pa_rows<T, D, 1><<<grid, kPaThreads, 0, st>>>(a);
+  pa_launch_merge<T, kPrRows, kPtRows>(a, st);
+  return record_launch();
 }
 
 static bool pa_sizes_ok(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D) {
   if (T < 0 || B < 0 || Hq < 0 || Hk <= 0 || D <= 0 || Hq % Hk != 0 || Hq > 65536) return false;
   return T <= INT_MAX && B < INT_MAX && T * Hq < (int64_t)1 << 31 && (std::min(B, T) + T * (Hq / Hk)) * Hk < (int64_t)1 << 24;
 }
-constexpr int64_t kPaTarget = 1024;
-// Rows of a tile. The workspace is sized for the MFMA kernels' tiles wherever dtype and head_dim allow them; a
-// call that turns out unaligned has smaller tiles.
-static int pa_tile(int dtype, int64_t D) { return dtype != AK_F32 && (D == 64 || D == 128) ? kPrRows : kPaRowTile; }
 
 }  // namespace ak
 
 using namespace ak;
 
+// The workspace is sized for the MFMA kernels wherever dtype and head_dim allow them; a call that turns out
+// unaligned needs less.
 extern "C" int64_t ak_paged_attn_workspace_bytes(int dtype, int64_t T, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                                                  int64_t page_size, int64_t max_pages) {
   if (dtype != AK_F32 && dtype != AK_F16 && dtype != AK_BF16) return 0;
   if (!pa_sizes_ok(T, B, Hq, Hkv, D) || T == 0 || B == 0 || Hq == 0 || page_size <= 0 || max_pages < 0) return 0;
   if (page_size > INT_MAX || max_pages > INT_MAX) return 0;
-  return pa_plan(T, B, Hq, Hkv, D, page_size * max_pages, pa_tile(dtype, D), kPaTarget).ws_bytes;
+  const bool fast = dtype != AK_F32 && (D == 64 || D == 128);
+  return std::max(pa_plan(T, B, Hq, Hkv, D, page_size, max_pages, fast).bytes(),
+                  pa_plan(T, B, Hq, Hkv, D, page_size, max_pages, false).bytes());
 }
 
 extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o,
@@ -667,8 +1099,7 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
   if (!q || !o || !q_strides || !o_strides || !k_cache_strides || !v_cache_strides) return AK_EINVAL;
   if (num_pages > 0 && (!k_cache || !v_cache)) return AK_EINVAL;
   if (!(sm_scale > 0.f) || sm_scale > 3e38f) return AK_EINVAL;
-  const int64_t keys = page_size * max_pages;
-  const int64_t need = pa_plan(T, B, Hq, Hkv, D, keys, pa_tile(dtype, D), kPaTarget).ws_bytes;
+  const int64_t need = ak_paged_attn_workspace_bytes(dtype, T, B, Hq, Hkv, D, page_size, max_pages);
   if (need > 0 && (!host_aligned16(workspace) || !workspace || workspace_bytes < need)) return AK_EINVAL;
   PaArgs a{};
   a.q = q, a.kc = k_cache, a.vc = v_cache, a.o = o;
@@ -683,16 +1114,18 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
   // K rows in 16-byte vectors
   const int vw = dtype == AK_F32 ? 4 : 8;
   a.vec = D % vw == 0 && host_aligned16(k_cache) && a.kcp % vw == 0 && a.kch % vw == 0 && a.kct % vw == 0;
-  bool mfma = a.vec && dtype != AK_F32 && (D == 64 || D == 128) && host_aligned16(v_cache) && host_aligned16(q) &&
+  bool fast = a.vec && dtype != AK_F32 && (D == 64 || D == 128) && host_aligned16(v_cache) && host_aligned16(q) &&
               host_aligned16(o);
   for (const int64_t x : {a.vcp, a.vch, a.vct, a.qst, a.qsh, a.ost, a.osh})
-    if (x % 8 != 0) mfma = false;
-  if (mfma) {
-    const PaPlan p = pa_plan(T, B, Hq, Hkv, D, keys, kPrRows, kPaTarget);
+    if (x % 8 != 0) fast = false;
+  // pa_tiles addresses up to 8 slots with 32 bits
+  for (const int64_t x : {a.kct, a.vct})
+    if (x < D || x > (1 << 24)) fast = false;
+  const PaPlan p = pa_plan(T, B, Hq, Hkv, D, page_size, max_pages, fast);
+  if (fast) {
     if (dtype == AK_F16)
-      return D == 64 ? launch_rows<TF16, 64>(a, p, workspace, stream) : launch_rows<TF16, 128>(a, p, workspace, stream);
-    return D == 64 ? launch_rows<TBF16, 64>(a, p, workspace, stream) : launch_rows<TBF16, 128>(a, p, workspace, stream);
+      return D == 64 ? launch_fast<TF16, 64>(a, p, workspace, stream) : launch_fast<TF16, 128>(a, p, workspace, stream);
+    return D == 64 ? launch_fast<TBF16, 64>(a, p, workspace, stream) : launch_fast<TBF16, 128>(a, p, workspace, stream);
   }
-  const PaPlan p = pa_plan(T, B, Hq, Hkv, D, keys, kPaRowTile, kPaTarget);
-  AK_DISPATCH(dtype, T_, return (pa_launch<T_, kPaRowTile>(pa_general<T_>, a, p, workspace, stream)));
+  AK_DISPATCH(dtype, T_, return launch_general<T_>(a, p, workspace, stream));
 }

@@ -239,13 +239,14 @@ def flash_attn_fwd(o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.T
          int(bool(causal)), float(sm_scale))
 
 
-_I64x2 = ctypes.c_int64 * 2
+_I64x2, _I64x4 = ctypes.c_int64 * 2, ctypes.c_int64 * 4
+_NO_STRIDES = _I64x2(0, 0)
 
 
 def _paged_sizes(k_cache: torch.Tensor, page_table: torch.Tensor) -> tuple:
     """(num_pages, page_size, max_pages, table_stride)"""
-    return (k_cache.shape[0], k_cache.shape[2], page_table.shape[1],
-            page_table.stride(0) if page_table.shape[0] > 1 else page_table.shape[1])
+    cache, (rows, width) = k_cache.shape, page_table.shape
+    return cache[0], cache[2], width, page_table.stride(0) if rows > 1 else width
 
 
 def kv_append(q_out: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.Tensor, q: torch.Tensor | None,
@@ -255,13 +256,12 @@ def kv_append(q_out: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.
     by the fp32 rows of cos / sin [rows, rot_dim / 2] (None: no rotation)."""
     T, Hkv, D = k.shape
     rows, rot = (0, 0) if cos is None else (cos.shape[0], 2 * cos.shape[1])
-    none = _I64x2(0, 0)
-    st = [none if t is None else _I64x2(*t.stride()[:2]) for t in (q, k, v, q_out)]
+    st = [_NO_STRIDES if t is None else _I64x3(*t.stride()) for t in (q, k, v, q_out)]
     _run("ak_kv_append", k, lambda: dict(k=tuple(k.shape), cache=tuple(k_cache.shape), dtype=k.dtype),
          _code(k, "kv_append"), _lib.ptr(q), k.data_ptr(), v.data_ptr(), _lib.ptr(q_out), k_cache.data_ptr(),
          v_cache.data_ptr(), _lib.ptr(cos), _lib.ptr(sin), page_table.data_ptr(), q_starts.data_ptr(),
          kv_lens.data_ptr(), T, kv_lens.shape[0], 0 if q is None else q.shape[1], Hkv, D, rot, rows,
-         *_paged_sizes(k_cache, page_table), *st, _I64x3(*k_cache.stride()[:3]), _I64x3(*v_cache.stride()[:3]),
+         *_paged_sizes(k_cache, page_table), *st, _I64x4(*k_cache.stride()), _I64x4(*v_cache.stride()),
          int(bool(interleaved)))
 
 
@@ -282,8 +282,8 @@ def paged_attn(o: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     ws = torch.empty(nbytes // 4, device=q.device, dtype=torch.float32) if nbytes > 0 else None
     _run("ak_paged_attn", q, lambda: dict(q=tuple(q.shape), cache=tuple(k_cache.shape), dtype=q.dtype), code,
          q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), page_table.data_ptr(),
-         q_starts.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, *sizes, _I64x2(*q.stride()[:2]),
-         _I64x3(*k_cache.stride()[:3]), _I64x3(*v_cache.stride()[:3]), _I64x2(*o.stride()[:2]), float(sm_scale),
+         q_starts.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, *sizes, _I64x3(*q.stride()),
+         _I64x4(*k_cache.stride()), _I64x4(*v_cache.stride()), _I64x3(*o.stride()), float(sm_scale),
          _lib.ptr(ws), nbytes)
 
 

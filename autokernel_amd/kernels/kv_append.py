@@ -31,11 +31,14 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
               page_table: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor,
               cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, q: torch.Tensor | None = None,
               interleaved: bool = True) -> torch.Tensor | None:
-    _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, k=k, v=v, q=q)
+    if q is None:
+        _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, k=k, v=v)
+    else:
+        _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, k=k, v=v, q=q)
     if k.shape[1] != k_cache.shape[1] or v.shape[1] != k_cache.shape[1]:
         raise ValueError(f"kv_append: k {tuple(k.shape)} and v {tuple(v.shape)} for {k_cache.shape[1]} KV heads")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"kv_append: {name} is an expanded view (strides {t.stride()}): its slots share memory")
     if (cos is None) != (sin is None):
         raise ValueError("kv_append: cos and sin come together")
@@ -43,9 +46,11 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         if q is not None:
             raise ValueError("kv_append: q without cos and sin has nothing done to it")
     else:
-        if not (cos.is_cuda and sin.is_cuda):
+        dev = k.get_device()
+        if cos.get_device() < 0 or sin.get_device() < 0:
             raise RuntimeError("kv_append: no CPU path (tensors must be on the GPU)")
-        if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != k.device or sin.device != k.device:
+        if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.get_device() != dev
+                or sin.get_device() != dev):
             raise ValueError(f"kv_append: cos and sin must be float32 on {k.device}")
         if cos.dim() != 2 or cos.shape != sin.shape or not 0 < 2 * cos.shape[1] <= k.shape[2]:
             raise ValueError(f"kv_append: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be "
@@ -55,6 +60,6 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
     q_out = None
     if q is not None:
         q = _paged.row_operand(q)
-        q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        q_out = q.new_empty(q.shape)
     _ops.kv_append(q_out, k_cache, v_cache, q, k, v, cos, sin, page_table, q_starts, kv_lens, interleaved)
     return q_out

@@ -34,7 +34,7 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
     if not 0.0 < scale < 3e38:
         raise ValueError(f"paged_attention: sm_scale {scale} must be positive and finite")
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        out = q.new_empty(q.shape)
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device
           or (out.shape[2] > 1 and out.stride(2) != 1)
           or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride()))):

@@ -450,3 +450,64 @@ def test_workspace_too_small_is_refused(gpu):
             _ops._run("ak_paged_attn", q, None, _lib.AK_BF16, q.data_ptr(), kc.data_ptr(), vc.data_ptr(), o.data_ptr(),
                       *(t.data_ptr() for t in b.index()), 1, 1, 4, 2, 64, b.pages, 8, b.width, b.width, st2, st3, st3, st2,
                       0.125, ptr, n)
+
+
+def _check_rows(q, kc, vc, table, starts, lens, out, rows, dtype):
+    """Some rows of a large call against 64-bit attention on the GPU (the bound of paged_oracle.attention)."""
+    H, D = q.shape[1:]
+    Hk, P = kc.shape[1:3]
+    G = H // Hk
+    st, ln = starts.tolist(), lens.tolist()
+    half = po.HALF[dtype]
+    for t in rows:
+        b = max(i for i in range(len(ln)) if st[i] <= t)
+        n = ln[b] - (st[b + 1] - t) + 1
+        ids = table[b, :-(-n // P)].long()
+        for hk in range(Hk):
+            K = kc[ids, hk].reshape(-1, D)[:n].double()
+            V = vc[ids, hk].reshape(-1, D)[:n].double()
+            x = q[t, hk * G:(hk + 1) * G].double()
+            s = x @ K.T.contiguous() * D ** -0.5
+            want = torch.softmax(s, -1) @ V
+            mag = (x.abs() @ K.abs().T.contiguous() * D ** -0.5).amax(-1, keepdim=True)
+            d = (D + 6) * 2.0 ** -24 * mag + 2.0 ** -21 + n * 2.0 ** -24 + (half if dtype != F32 else 0)
+            tol = 2 * d * V.abs().amax(0, keepdim=True) + half * want.abs() + po.TINY[dtype]
+            got = out[t, hk * G:(hk + 1) * G].double()
+            assert ((got - want).abs() <= tol).all(), (t, hk, (got - want).abs().max())
+
+
+@pytest.mark.parametrize("heads,kv_heads,D,page,chunks,lens", [
+    (32, 2, 64, 8, [1024], [40000]),            # page numbers of a slice past the ring that holds them
+    (8, 8, 128, 16, [2100, 1, 130], [2100, 5000, 9000]),
+    (32, 8, 128, 32, [512], [16513]),
+    (16, 1, 128, 8, [700, 3], [30000, 70]),
+])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_large_chunks(gpu, dtype, heads, kv_heads, D, page, chunks, lens):
+    print(f"paged_attention large {heads}/{kv_heads} {D} page {page} {chunks} {lens} {dtype}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    need = [-(-n // page) for n in lens]
+    pages = sum(need) + 1
+    kc, vc = ((torch.randn(pages, kv_heads, page, D, generator=g, device="cuda")).to(dtype) for _ in range(2))
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.zeros(len(lens), max(need), dtype=torch.int32, device="cuda")
+    at = 0
+    for b, c in enumerate(need):
+        table[b, :c] = order[at:at + c]
+        at += c
+    starts = torch.tensor([0] + torch.tensor(chunks).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    T = int(starts[-1])
+    q = torch.randn(T, heads, D, generator=g, device="cuda").to(dtype)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = attn(q, kc, vc, table, starts, ln)
+    picks = {0, 1, 31, 32, T // 2, T - 2, T - 1} | set(torch.randint(0, T, (12,)).tolist()) | {int(x) for x in starts[:-1]}
+    _check_rows(q, kc, vc, table, starts, ln, out, sorted(picks), dtype)
+    assert torch.equal(_bits(out), _bits(attn(q, kc, vc, table, starts, ln)))
+
+
+def test_attention_a_sequence_alone_or_in_a_batch(gpu):
+    """Chunks beside single tokens (both tile sizes in one launch): each sequence within its own bound."""
+    b = po.Batch([1, 200, 16, 17, 1, 65, 64, 1], [700, 1000, 16, 300, 1, 65, 2000, 64], 8, 2, 128, 16, BF16, seed=2, pad=5)
+    _check_attn(b, "mixed")
+    b = po.Batch([1, 200, 64, 65, 1, 130, 1], [700, 1000, 64, 300, 1, 130, 64], 4, 4, 64, 8, F16, seed=3, pad=1)
+    _check_attn(b, "mixed")
