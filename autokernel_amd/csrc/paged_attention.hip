@@ -46,6 +46,8 @@ struct PaArgs {
   PagedSeqs s;
 };
 
+__device__ __forceinline__ int pa_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 struct PaSeq {
   int t0, n, len;   // first row, rows, cached tokens (new ones among them)
   bool overlong;    // longer than its page table: NaN rows
@@ -124,16 +126,17 @@ __device__ __forceinline__ bool pa_find(const PaArgs& a, uint32_t it, PaItem& o)
       o.b = i + l;
       tiles = __builtin_amdgcn_readlane(tiles, l);
       o.seq = pa_seq(a.s, o.b);
-      o.seq.t0 = __builtin_amdgcn_readfirstlane(o.seq.t0);  // one sequence: keep it in scalar registers
-      o.seq.n = __builtin_amdgcn_readfirstlane(o.seq.n);
-      o.seq.len = __builtin_amdgcn_readfirstlane(o.seq.len);
-      o.chunk = __builtin_amdgcn_readfirstlane(o.chunk);
-      o.nsplit = pa_splits(o.seq.len, o.chunk);
+      // one sequence for the whole block: what is made from it belongs in scalar registers
+      o.seq.t0 = pa_uniform(o.seq.t0);
+      o.seq.n = pa_uniform(o.seq.n);
+      o.seq.len = pa_uniform(o.seq.len);
+      o.chunk = pa_uniform(o.chunk);
+      o.nsplit = pa_uniform(pa_splits(o.seq.len, o.chunk));
       const uint32_t rel = it - base - (uint32_t)__builtin_amdgcn_readlane(inc - cnt, l);
       const uint32_t x = fdiv(rel, a.f_hk);
-      o.hk = (int)(rel - x * a.Hk);
-      o.split = (int)(x / (uint32_t)tiles);
-      o.tile = tiles - 1 - (int)(x - (uint32_t)o.split * tiles);
+      o.hk = pa_uniform((int)(rel - x * a.Hk));
+      o.split = pa_uniform((int)(x / (uint32_t)tiles));
+      o.tile = pa_uniform(tiles - 1 - (int)(x - (uint32_t)o.split * tiles));
       return o.split < o.nsplit;
     }
     base += (uint32_t)__builtin_amdgcn_readlane(inc, kWave - 1);
@@ -418,7 +421,7 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
   const uint16_t* Kb = (const uint16_t*)a.kc + it.hk * a.kch + g * 8;
   const uint16_t* Vb = (const uint16_t*)a.vc + it.hk * a.vch + i16 * VW;
   const int rows = it.seq.n * a.G, r0 = it.tile * kPrRows, r = r0 + i16;
-  const int lim = r < rows ? (int)pa_seen(it, r, a.f_g) : 0;  // keys that this lane's row sees
+  const int lim = r < rows ? pa_seen(it, r, a.f_g) : 0;  // keys that this lane's row sees
   u32x4 qf[NS];
   {
     const int tk = (int)fdiv((uint32_t)min(r, rows - 1), a.f_g);
@@ -428,9 +431,9 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
     for (int s = 0; s < NS; ++s) qf[s] = r < rows ? ld16(q + s * 32 + g * 8) : u32x4{0u, 0u, 0u, 0u};
   }
   const int rl = min(rows, r0 + kPrRows) - 1;  // the tile's last row sees the most
-  const int kbeg = it.nsplit == 1 ? 0 : it.split * it.chunk;
-  const int kend = min((int)pa_seen(it, rl, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk);
-  const int full = (int)pa_seen(it, r0, a.f_g);  // every row sees the keys below
+  const int kbeg = pa_uniform(it.nsplit == 1 ? 0 : it.split * it.chunk);
+  const int kend = pa_uniform(min(pa_seen(it, rl, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk));
+  const int full = pa_uniform(pa_seen(it, r0, a.f_g));  // every row sees the keys below
 
   struct Pages {
     int k[NK], v[NV];
@@ -531,7 +534,7 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
   };
 
   constexpr int kStride = kPaWaves * kPrKeys;
-  int k0 = kbeg + w * kPrKeys;
+  int k0 = kbeg + pa_uniform(w) * kPrKeys;
   if (k0 < kend) {
     Step s0, s1;
     Pages p0, p1;
@@ -635,6 +638,9 @@ __device__ __forceinline__ void pa_dma16(const u32x4& rsrc, uint32_t voff, uint3
       : "v"(voff), "s"(rsrc), "{m0}"(lds)
       : "memory");
 }
+// fdiv for divisors of 8 and more: its shift is past the low word
+__device__ __forceinline__ uint32_t pt_div(uint32_t n, FastDiv f) { return __umulhi(n, f.m) >> (f.s - 1); }
+
 template <int D>
 struct PtShared {
   uint16_t k[2 * kFaBKV * D], v[2 * kFaBKV * D];
@@ -655,11 +661,12 @@ __device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, Pt
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const int rows = it.seq.n * a.G, r0 = it.tile * kPtRows, rw0 = r0 + 32 * w;  // this wave's first row
   const int my_r = rw0 + l32;
-  const int kbeg = it.nsplit == 1 ? 0 : it.split * it.chunk;
-  const int kend = min(pa_seen(it, min(rows, r0 + kPtRows) - 1, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk);
+  const int kbeg = pa_uniform(it.nsplit == 1 ? 0 : it.split * it.chunk);
+  const int kend = pa_uniform(
+      min(pa_seen(it, min(rows, r0 + kPtRows) - 1, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk));
   const int tk = (int)fdiv((uint32_t)min(my_r, rows - 1), a.f_g);
   const int64_t head = it.hk * a.G + min(my_r, rows - 1) - tk * a.G, tok = it.seq.t0 + tk;
-  const int nt = (max(kend - kbeg, 0) + kFaBKV - 1) / kFaBKV;
+  const int nt = pa_uniform((max(kend - kbeg, 0) + kFaBKV - 1) / kFaBKV);
   float m_run = -INFINITY, l_run = 0.f;
   f32x16 o[NDB];
 #pragma unroll
@@ -671,15 +678,15 @@ __device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, Pt
   if (nt > 0) {
     // keys seen by this lane's row, by the wave's first row and by its last
     const int lim = min(pa_seen(it, min(my_r, rows - 1), a.f_g), kend);
-    const int lim0 = min(pa_seen(it, min(rw0, rows - 1), a.f_g), kend);
-    const int lim1 = min(pa_seen(it, min(rw0 + 31, rows - 1), a.f_g), kend);
-    const int jw = rw0 < rows && lim1 > kbeg ? (lim1 - 1 - kbeg) / kFaBKV : -1;  // the wave's last tile
+    const int lim0 = pa_uniform(min(pa_seen(it, min(rw0, rows - 1), a.f_g), kend));
+    const int lim1 = pa_uniform(min(pa_seen(it, min(rw0 + 31, rows - 1), a.f_g), kend));
+    const int jw = pa_uniform(rw0 < rows && lim1 > kbeg ? (lim1 - 1 - kbeg) / kFaBKV : -1);  // the wave's last tile
 
     // page numbers kbeg / page_size .. (kend - 1) / page_size, entry e at e % kPtWin
     const int32_t* tab = a.s.table + it.b * a.s.table_stride;
-    const int e_last = (int)fdiv((uint32_t)(kend - 1), a.s.page_div);
+    const int e_last = pa_uniform((int)fdiv((uint32_t)(kend - 1), a.s.page_div));
     constexpr int kHalf = kPtWin / 2;
-    int half = (int)fdiv((uint32_t)kbeg, a.s.page_div) / kHalf;  // the half that V's transfers have come to
+    int half = pa_uniform((int)fdiv((uint32_t)kbeg, a.s.page_div) / kHalf);  // the half that V's transfers have come to
     auto fill = [&](int h) {
       for (int e = h * kHalf + (int)threadIdx.x; e < (h + 1) * kHalf && e <= e_last; e += kPaThreads)
         sh.page[e % kPtWin] = tab[e];
@@ -687,58 +694,57 @@ __device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, Pt
     fill(half);
     fill(half + 1);
     __syncthreads();
-    auto page_of = [&](int j) {  // lane i % NIW: page number of transfer i of tile j
-      const int key = min(kbeg + j * kFaBKV + ((lane & (NIW - 1)) * kPaWaves + w) * RPI, kend - 1);
-      return sh.page[fdiv((uint32_t)key, a.s.page_div) % kPtWin];
-    };
 
     const uint16_t* Qr = (const uint16_t*)a.q + tok * a.qst + head * a.qsh;
     u32x4 qf[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) qf[s] = my_r < rows ? ld16(Qr + s * 16 + hh * 8) : u32x4{0u, 0u, 0u, 0u};
 
-    // Byte offsets of a lane inside a transfer: lane L writes physical chunk L % DC of row L / DC and so
-    // fetches the logical chunk that the swizzle maps there.
-    uint32_t offk[NIW], offv[NIW];
-#pragma unroll
-    for (int i = 0; i < NIW; ++i) {
-      const int row = (i * kPaWaves + w) * RPI + lane / DC, pc = lane % DC;
-      offk[i] = (uint32_t)((lane / DC) * (int)a.kct * 2 + ((pc ^ fa2_kswz<D>(row)) * 16));
-      offv[i] = (uint32_t)((lane / DC) * (int)a.vct * 2 + ((pc ^ fa2_vswz<D>(row)) * 16));
-    }
+    // Byte offset of a lane inside a transfer: lane L writes physical chunk L % DC of row L / DC and so fetches
+    // the logical chunk that the swizzle maps there. (A wave's transfers start at rows that the swizzles do not
+    // tell apart.)
+    const int srow = w * RPI + lane / DC;
+    const uint32_t offk = (uint32_t)((lane / DC) * (int)a.kct * 2 + (((lane % DC) ^ fa2_kswz<D>(srow)) * 16));
+    const uint32_t offv = (uint32_t)((lane / DC) * (int)a.vct * 2 + (((lane % DC) ^ fa2_vswz<D>(srow)) * 16));
     const uint32_t sK_lds = (uint32_t)(uintptr_t)(lds_void*)sh.k, sV_lds = (uint32_t)(uintptr_t)(lds_void*)sh.v;
-    auto issue = [&](const uint16_t* base, int64_t ps, int64_t ss, const uint32_t (&off)[NIW], int pages, int j,
+    // Lane i % NIW prepares transfer i of a tile, all transfers side by side: address and bytes of its keys.
+    // (Made by the scalar unit one transfer after another, 35 instructions each, they cost a third of the
+    // kernel's time.)
+    const int koff = kbeg + ((lane & (NIW - 1)) * kPaWaves + w) * RPI;
+    auto entry = [&](int j) { return pt_div((uint32_t)min(j * kFaBKV + koff, kend - 1), a.s.page_div); };
+    auto issue = [&](const uint16_t* base, uint32_t page_bytes, uint32_t slot_bytes, uint32_t off, int page, int j,
                      uint32_t lds) {
+      const int key = j * kFaBKV + koff, left = min(kend - key, RPI);
+      const uint32_t slot = (uint32_t)key - pt_div((uint32_t)key, a.s.page_div) * (uint32_t)a.s.page_size;
+      const bool in = (uint32_t)page < (uint32_t)a.s.num_pages, any = left > 0;
+      bad |= any && !in;
+      const uint64_t at = (uint64_t)(uintptr_t)base + (uint64_t)(uint32_t)page * page_bytes + (uint64_t)slot * slot_bytes;
+      const uint32_t lo = (uint32_t)at, hi = (uint32_t)(at >> 32) & 0xffffu;
+      const uint32_t n = any && in ? (uint32_t)(left - 1) * slot_bytes + D * 2 : 0u;
 #pragma unroll
       for (int i = 0; i < NIW; ++i) {
-        const int key = kbeg + j * kFaBKV + (i * kPaWaves + w) * RPI;
-        const int left = min(kend - key, RPI);
-        const int pg = __builtin_amdgcn_readlane(pages, i);
-        const int slot = key - (int)fdiv((uint32_t)key, a.s.page_div) * a.s.page_size;
-        const bool in = (uint32_t)pg < a.s.num_pages;
-        bad |= !in && left > 0;
-        const u32x4 rs = fa2_rsrc(in ? base + pg * ps + slot * ss : base,
-                                  in && left > 0 ? (uint32_t)(((left - 1) * (int)ss + D) * 2) : 0u);
-        pa_dma16(rs, off[i], lds + (i * kPaWaves + w) * 1024);
+        const u32x4 rs = {(uint32_t)__builtin_amdgcn_readlane((int)lo, i), (uint32_t)__builtin_amdgcn_readlane((int)hi, i),
+                          (uint32_t)__builtin_amdgcn_readlane((int)n, i), 0x00020000u};
+        pa_dma16(rs, off, lds + (i * kPaWaves + w) * 1024);
       }
     };
     const uint16_t* Kb = (const uint16_t*)a.kc + it.hk * a.kch;
     const uint16_t* Vb = (const uint16_t*)a.vc + it.hk * a.vch;
-    int pk = page_of(0), pv_ = pk;  // page numbers of the next K and V tile to be issued
+    int pk = sh.page[entry(0) % kPtWin], pv_ = pk;  // page numbers of the next K and V tile to be issued
     auto issue_k = [&](int j, int stage) {
-      issue(Kb, a.kcp, a.kct, offk, pk, j, sK_lds + stage * TILE * 2);
-      pk = page_of(j + 1);
+      issue(Kb, (uint32_t)a.kcp * 2, (uint32_t)a.kct * 2, offk, pk, j, sK_lds + stage * TILE * 2);
+      pk = sh.page[entry(j + 1) % kPtWin];
     };
     auto issue_v = [&](int j, int stage) {
-      issue(Vb, a.vcp, a.vct, offv, pv_, j, sV_lds + stage * TILE * 2);
-      const int h = (int)fdiv((uint32_t)(kbeg + j * kFaBKV), a.s.page_div) / kHalf;
+      issue(Vb, (uint32_t)a.vcp * 2, (uint32_t)a.vct * 2, offv, pv_, j, sV_lds + stage * TILE * 2);
+      const int h = pa_uniform((int)(pt_div((uint32_t)(kbeg + j * kFaBKV), a.s.page_div) / kHalf));
       // every wave's V numbers of this half's tiles on come from this half or the next, every K number read so
       // far too: the half behind can take the one after
       if (h > half) {
         half = h;
         fill(half + 1);
       }
-      pv_ = page_of(j + 1);
+      pv_ = sh.page[entry(j + 1) % kPtWin];
     };
 
     auto qk = [&](const uint16_t* ks, f32x16 (&s)[2]) {
@@ -1118,9 +1124,11 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
               host_aligned16(o);
   for (const int64_t x : {a.vcp, a.vch, a.vct, a.qst, a.qsh, a.ost, a.osh})
     if (x % 8 != 0) fast = false;
-  // pa_tiles addresses up to 8 slots with 32 bits
+  // pa_tiles addresses inside a page with 32 bits
   for (const int64_t x : {a.kct, a.vct})
-    if (x < D || x > (1 << 24)) fast = false;
+    if (x < D || x > (1 << 24) || x * page_size >= (int64_t)1 << 31) fast = false;
+  for (const int64_t x : {a.kcp, a.vcp})
+    if (x < 0 || x >= (int64_t)1 << 31) fast = false;
   const PaPlan p = pa_plan(T, B, Hq, Hkv, D, page_size, max_pages, fast);
   if (fast) {
     if (dtype == AK_F16)
