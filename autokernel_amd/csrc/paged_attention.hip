@@ -85,19 +85,31 @@ __device__ __forceinline__ int pa_tiles_of(const PaArgs& a, const PaSeq& q) {
   const int rows = q.n * a.G;
   return (CLS == 0) == (rows <= a.split_rows) ? (rows + BM - 1) / BM : 0;
 }
+// The batch, one sequence a lane: a call of up to 64 sequences reads its lengths once.
+struct PaBatch {
+  PaSeq q;  // sequence lane_id() (no rows past the last)
+};
+__device__ __forceinline__ PaSeq pa_lane_seq(const PagedSeqs& s, int b) {
+  return b < s.B ? pa_seq(s, b) : PaSeq{0, 0, 0, false};
+}
+// f(first sequence of 64, this lane's sequence) until it returns true
+template <typename F>
+__device__ __forceinline__ void pa_each(const PaArgs& a, const PaBatch& x, F f) {
+  if (f(0, x.q)) return;
+  for (int i = kWave; i < a.s.B; i += kWave)
+    if (f(i, pa_lane_seq(a.s, i + lane_id()))) return;
+}
 template <int BM, int CLS>
-__device__ __forceinline__ int pa_chunk(const PaArgs& a) {
+__device__ __forceinline__ int pa_chunk(const PaArgs& a, const PaBatch& x) {
   if (a.c[CLS].target <= 0.f) return INT_MAX;
   float w = 0.f;
-  for (int i = 0; i < a.s.B; i += kWave) {
-    const int b = i + lane_id();
-    if (b >= a.s.B) break;
-    const PaSeq q = pa_seq(a.s, b);
+  pa_each(a, x, [&](int, const PaSeq& q) {
     w += (float)pa_tiles_of<BM, CLS>(a, q) * (float)q.len;
-  }
+    return false;
+  });
   w = wave_sum(w) * (float)a.Hk * 1.001f;
   const float c = ceilf(w / a.c[CLS].target / (float)kPaSlice) * (float)kPaSlice;
-  return c >= 1e9f ? INT_MAX : max((int)c, kPaSlice);
+  return pa_uniform(c >= 1e9f ? INT_MAX : max((int)c, kPaSlice));
 }
 __device__ __forceinline__ int pa_splits(int len, int chunk) {
   return chunk == INT_MAX ? 1 : max(1, (len + chunk - 1) / chunk);
@@ -108,40 +120,37 @@ __device__ __forceinline__ int pa_splits(int len, int chunk) {
 // the most keys), then slices.
 template <int BM, int CLS>
 __device__ __forceinline__ bool pa_find(const PaArgs& a, uint32_t it, PaItem& o) {
-  o.chunk = pa_chunk<BM, CLS>(a);
+  const PaBatch x{pa_lane_seq(a.s, lane_id())};
+  o.chunk = pa_chunk<BM, CLS>(a, x);
   o.slot = it;
+  o.split = o.nsplit = 0;
   uint32_t base = 0;
-  for (int i = 0; i < a.s.B; i += kWave) {
-    const int b = i + lane_id();
-    int cnt = 0, tiles = 0;
-    if (b < a.s.B) {
-      const PaSeq q = pa_seq(a.s, b);
-      tiles = pa_tiles_of<BM, CLS>(a, q);
-      cnt = tiles * a.Hk * pa_splits(q.len, o.chunk);
-    }
+  pa_each(a, x, [&](int i, const PaSeq& q) {
+    int tiles = pa_tiles_of<BM, CLS>(a, q);
+    const int splits = pa_splits(q.len, o.chunk), cnt = tiles * a.Hk * splits;
     const int inc = pa_wave_scan(cnt);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(it - base < (uint32_t)inc && cnt > 0);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      o.b = i + l;
-      tiles = __builtin_amdgcn_readlane(tiles, l);
-      o.seq = pa_seq(a.s, o.b);
-      // one sequence for the whole block: what is made from it belongs in scalar registers
-      o.seq.t0 = pa_uniform(o.seq.t0);
-      o.seq.n = pa_uniform(o.seq.n);
-      o.seq.len = pa_uniform(o.seq.len);
-      o.chunk = pa_uniform(o.chunk);
-      o.nsplit = pa_uniform(pa_splits(o.seq.len, o.chunk));
-      const uint32_t rel = it - base - (uint32_t)__builtin_amdgcn_readlane(inc - cnt, l);
-      const uint32_t x = fdiv(rel, a.f_hk);
-      o.hk = pa_uniform((int)(rel - x * a.Hk));
-      o.split = pa_uniform((int)(x / (uint32_t)tiles));
-      o.tile = pa_uniform(tiles - 1 - (int)(x - (uint32_t)o.split * tiles));
-      return o.split < o.nsplit;
+    if (!hit) {
+      base += (uint32_t)__builtin_amdgcn_readlane(inc, kWave - 1);
+      return false;
     }
-    base += (uint32_t)__builtin_amdgcn_readlane(inc, kWave - 1);
-  }
-  return false;
+    // one sequence for the whole block: what is made from it belongs in scalar registers
+    const int l = __builtin_ctzll(hit);
+    o.b = i + l;
+    tiles = __builtin_amdgcn_readlane(tiles, l);
+    o.seq.t0 = __builtin_amdgcn_readlane(q.t0, l);
+    o.seq.n = __builtin_amdgcn_readlane(q.n, l);
+    o.seq.len = __builtin_amdgcn_readlane(q.len, l);
+    o.seq.overlong = __builtin_amdgcn_readlane((int)q.overlong, l) != 0;
+    o.nsplit = __builtin_amdgcn_readlane(splits, l);
+    const uint32_t rel = it - base - (uint32_t)__builtin_amdgcn_readlane(inc - cnt, l);
+    const uint32_t y = fdiv(rel, a.f_hk);
+    o.hk = pa_uniform((int)(rel - y * a.Hk));
+    o.split = pa_uniform((int)(y / (uint32_t)tiles));
+    o.tile = pa_uniform(tiles - 1 - (int)(y - (uint32_t)o.split * tiles));
+    return true;
+  });
+  return o.split < o.nsplit;
 }
 
 // Keys [lo, hi) of one row, by one wave: exact about what a row sees, whatever the rest of its pages hold.
@@ -271,103 +280,124 @@ __global__ __launch_bounds__(kPaThreads) void pa_general(const PaArgs a) {
 
 // Sliced rows: W waves per (row, query head). A group of 16 lanes adds the partials of slices g, g + 4 W, ..
 // (lane c: dims 4 c .. 4 c + 3 of each 64), then the groups' sums combine in group order. Four groups of one
-// wave for many rows; with few rows sixteen, so that 64 slices' partials are in flight at once.
+// wave for many rows; with few rows sixteen, so that 64 slices' partials are in flight at once. The grid is
+// bounded and walks the rows: in most calls with many rows nothing is sliced and it ends at once.
 template <typename T, int BM0, int BM1, int W>
 __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
   using S = typename T::S;
   constexpr int NG = 4 * W, NR = kPaWaves / W;  // groups of a row, rows of a block
   __shared__ float so[kPaWaves * 4][260], sm[kPaWaves * 4], sl[kPaWaves * 4];
   const int lane = lane_id(), c = lane & 15;
-  const int slot_in = wave_id() / W, g = (wave_id() % W) * 4 + lane / 16;
-  const int64_t row = (int64_t)blockIdx.x * NR + slot_in;
-  const int64_t tok = row / a.Hq;
-  const int h = (int)(row - tok * a.Hq);
-  PaSeq q{0, 0, 0, false};
-  int b = a.s.B, nsplit = 1, chunk = 0;
-  if (tok < a.s.T) b = paged_seq_of(a.s, (int)tok);
-  if (b < a.s.B) {
-    q = pa_seq(a.s, b);
-    if (tok >= q.t0 && tok < q.t0 + q.n) {
-      chunk = q.n * a.G <= a.split_rows ? pa_chunk<BM0, 0>(a) : pa_chunk<BM1, 1>(a);
-      nsplit = pa_splits(q.len, chunk);
-    }
-  }
-  const int cls = q.n * a.G <= a.split_rows ? 0 : 1, bm = cls ? BM1 : BM0;
-  const PaClass& cl = a.c[cls];
-  float m = -INFINITY, l = 0.f, acc[4][4];
+  const int slot_in = pa_uniform(wave_id()) / W, g = (wave_id() % W) * 4 + lane / 16;
+  const PaBatch x{pa_lane_seq(a.s, lane)};
+  const int chunk0 = pa_chunk<BM0, 0>(a, x), chunk1 = pa_chunk<BM1, 1>(a, x);
+  bool sliced = false;
+  pa_each(a, x, [&](int, const PaSeq& q) {
+    const int rows = q.n * a.G;
+    sliced = __builtin_amdgcn_ballot_w64(rows > 0 && pa_splits(q.len, rows <= a.split_rows ? chunk0 : chunk1) > 1) != 0;
+    return sliced;
+  });
+  if (!sliced) return;
+  const int64_t total = (int64_t)a.s.T * a.Hq;
+  for (int64_t block = blockIdx.x; block * NR < total; block += gridDim.x) {
+    const int64_t row = block * NR + slot_in;
+    const int tok = (int)(row / a.Hq), h = (int)(row - (int64_t)tok * a.Hq);
+    // the row's sequence, and the items of its class before it
+    PaSeq q{0, 0, 0, false};
+    int cls = 0, nsplit = 1;
+    uint32_t first = 0, before[2] = {0, 0};
+    if (row < total)
+      pa_each(a, x, [&](int, const PaSeq& s) {
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(tok >= s.t0 && tok < s.t0 + s.n);
+        const int n0 = pa_tiles_of<BM0, 0>(a, s) * a.Hk * pa_splits(s.len, chunk0);
+        const int n1 = pa_tiles_of<BM1, 1>(a, s) * a.Hk * pa_splits(s.len, chunk1);
+        const int i0 = pa_wave_scan(n0), i1 = pa_wave_scan(n1);
+        if (!hit) {
+          before[0] += (uint32_t)__builtin_amdgcn_readlane(i0, kWave - 1);
+          before[1] += (uint32_t)__builtin_amdgcn_readlane(i1, kWave - 1);
+          return false;
+        }
+        const int l = __builtin_ctzll(hit);
+        q.t0 = __builtin_amdgcn_readlane(s.t0, l);
+        q.n = __builtin_amdgcn_readlane(s.n, l);
+        q.len = __builtin_amdgcn_readlane(s.len, l);
+        q.overlong = __builtin_amdgcn_readlane((int)s.overlong, l) != 0;
+        cls = q.n * a.G <= a.split_rows ? 0 : 1;
+        nsplit = pa_splits(q.len, cls ? chunk1 : chunk0);
+        first = before[cls] + (uint32_t)__builtin_amdgcn_readlane(cls ? i1 - n1 : i0 - n0, l);
+        return true;
+      });
+    const int bm = cls ? BM1 : BM0;
+    const PaClass& cl = a.c[cls];
+    float m = -INFINITY, l = 0.f, acc[4][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-  if (nsplit > 1) {
-    // items of the sequences before this one
-    int first = 0;
-    for (int i = lane; i < b; i += kWave) {
-      const PaSeq x = pa_seq(a.s, i);
-      first += (cls ? pa_tiles_of<BM1, 1>(a, x) : pa_tiles_of<BM0, 0>(a, x)) * a.Hk * pa_splits(x.len, chunk);
-    }
-    first = __builtin_amdgcn_readlane(pa_wave_scan(first), kWave - 1);
-    const int tiles = (q.n * a.G + bm - 1) / bm;
-    const int hk = h / a.G, r = ((int)tok - q.t0) * a.G + h % a.G;
-    const uint32_t it0 = (uint32_t)first + (uint32_t)(tiles - 1 - r / bm) * a.Hk + hk;
-    for (int sp = g; sp < nsplit; sp += 4 * NG) {
-      float ms[4], ls[4];
-      f32x4 v[4][4];
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
+    if (nsplit > 1) {
+      const int tiles = (q.n * a.G + bm - 1) / bm;
+      const int hk = h / a.G, r = (tok - q.t0) * a.G + h % a.G;
+      const uint32_t it0 = first + (uint32_t)(tiles - 1 - r / bm) * a.Hk + hk;
+      for (int sp = g; sp < nsplit; sp += 4 * NG) {
+        float ms[4], ls[4];
+        f32x4 v[4][4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint32_t it = it0 + (uint32_t)(sp + u * NG) * tiles * a.Hk;
-        ms[u] = -INFINITY;
-        ls[u] = 0.f;
-        if (sp + u * NG >= nsplit || it >= cl.items) continue;
-        const int64_t slot = (int64_t)it * bm + r % bm;
-        ms[u] = cl.stat[slot * 2];
-        ls[u] = cl.stat[slot * 2 + 1];
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t it = it0 + (uint32_t)(sp + u * NG) * tiles * a.Hk;
+          ms[u] = -INFINITY;
+          ls[u] = 0.f;
+          if (sp + u * NG >= nsplit || it >= cl.items) continue;
+          const int64_t slot = (int64_t)it * bm + r % bm;
+          ms[u] = cl.stat[slot * 2];
+          ls[u] = cl.stat[slot * 2 + 1];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (64 * j + 4 * c < a.D) v[u][j] = *reinterpret_cast<const f32x4*>(cl.part + slot * a.Dp + 64 * j + 4 * c);
+          for (int j = 0; j < 4; ++j)
+            if (64 * j + 4 * c < a.D) v[u][j] = *reinterpret_cast<const f32x4*>(cl.part + slot * a.Dp + 64 * j + 4 * c);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (ms[u] == -INFINITY && ls[u] == 0.f) continue;  // a slice without a key that the row sees
+          const float m_new = nan_max(m, ms[u]);
+          const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+          const float f1 = ms[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[u] - m_new);
+          m = m_new;
+          l = l * f0 + ls[u] * f1;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (64 * j + 4 * c < a.D)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] * f0 + v[u][j][e] * f1;
+        }
       }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (ms[u] == -INFINITY && ls[u] == 0.f) continue;  // a slice without a key that the row sees
-        const float m_new = nan_max(m, ms[u]);
-        const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-        const float f1 = ms[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[u] - m_new);
-        m = m_new;
-        l = l * f0 + ls[u] * f1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (64 * j + 4 * c < a.D)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] * f0 + v[u][j][e] * f1;
-      }
     }
-  }
-  const int me = slot_in * NG + g;
+    const int me = slot_in * NG + g;
+    __syncthreads();  // the block's last rows have been read
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (64 * j + 4 * c < a.D) *reinterpret_cast<f32x4*>(&so[me][64 * j + 4 * c]) = f32x4{acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
-  if (c == 0) {
-    sm[me] = m;
-    sl[me] = l;
-  }
-  __syncthreads();
-  if (nsplit == 1) return;
-  float mb = -INFINITY, lb = 0.f;
-  for (int x = 0; x < NG; ++x) mb = nan_max(mb, sm[slot_in * NG + x]);
-  float f[NG];
+    for (int j = 0; j < 4; ++j)
+      if (64 * j + 4 * c < a.D)
+        *reinterpret_cast<f32x4*>(&so[me][64 * j + 4 * c]) = f32x4{acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
+    if (c == 0) {
+      sm[me] = m;
+      sl[me] = l;
+    }
+    __syncthreads();
+    if (nsplit == 1) continue;
+    float mb = -INFINITY, lb = 0.f, f[NG];
+    for (int y = 0; y < NG; ++y) mb = nan_max(mb, sm[slot_in * NG + y]);
 #pragma unroll
-  for (int x = 0; x < NG; ++x) {
-    const float mx = sm[slot_in * NG + x];
-    f[x] = mx == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mx - mb);
-    lb += sl[slot_in * NG + x] * f[x];
-  }
-  const float inv = pa_inv(q, q.len - (q.t0 + q.n - (int)tok) >= 0, lb);  // its position
-  S* o = (S*)a.o + tok * a.ost + h * a.osh;
-  for (int d = (wave_id() % W) * kWave + lane; d < a.D; d += W * kWave) {
-    float v = 0.f;
+    for (int y = 0; y < NG; ++y) {
+      const float my = sm[slot_in * NG + y];
+      f[y] = my == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(my - mb);
+      lb += sl[slot_in * NG + y] * f[y];
+    }
+    const float inv = pa_inv(q, q.len - (q.t0 + q.n - tok) >= 0, lb);  // its position
+    S* o = (S*)a.o + (int64_t)tok * a.ost + (int64_t)h * a.osh;
+    for (int d = (wave_id() % W) * kWave + lane; d < a.D; d += W * kWave) {
+      float v = 0.f;
 #pragma unroll
-    for (int x = 0; x < NG; ++x) v += so[slot_in * NG + x][d] * f[x];
-    o[d] = T::from_f(v * inv);
+      for (int y = 0; y < NG; ++y) v += so[slot_in * NG + y][d] * f[y];
+      o[d] = T::from_f(v * inv);
+    }
   }
 }
 
@@ -1049,7 +1079,7 @@ static void pa_launch_merge(const PaArgs& a, hipStream_t st) {
   if (a.c[0].target <= 0.f && a.c[1].target <= 0.f) return;
   const int64_t rows = (int64_t)a.s.T * a.Hq;
   if (rows <= 4096) pa_merge<T, BM0, BM1, 4><<<dim3((unsigned)rows), kPaThreads, 0, st>>>(a);
-  else pa_merge<T, BM0, BM1, 1><<<dim3((unsigned)cdiv(rows, kPaWaves)), kPaThreads, 0, st>>>(a);
+  else pa_merge<T, BM0, BM1, 1><<<dim3((unsigned)std::min<int64_t>(cdiv(rows, kPaWaves), 2048)), kPaThreads, 0, st>>>(a);
 }
 template <typename T>
 static int launch_general(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
