@@ -648,14 +648,13 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
 // read transposed by ds_read_b64_tr_b16, each MFMA burst beside the other product's softmax work, the
 // lazily raised exp2 base). What is different:
 //   * A row is a (token, head of the group) pair, so the query heads of a KV head share its K and V tiles.
-//   * A DMA transfer covers 4 (head_dim 128) or 8 (64) keys and so, with pages of a multiple of 8 slots, lies
-//     in one page: a wave makes each transfer's buffer resource from that page's address, with as many
-//     bytes as the page has keys of the slice left (the rest arrives as zeros). The slice's page numbers wait in
-//     LDS (a ring of kPtWin, refilled by halves), read one tile ahead.
+//   * A wave brings 16 consecutive keys of a tile, which with pages of a multiple of 16 slots lie in one page,
+//     through a buffer resource of that page's address and as many bytes as the slice has keys left there (the
+//     rest arrives as zeros). The resources of 64 tiles are made at once, one per lane.
 //   * No pass over what a row does not see: V of masked keys only has to be finite. Where a row's result is
 //     NaN, or a page lies outside the cache, the item's rows are computed again by pa_row.
 // Bound by the MFMA and the softmax VALU work, as fa_fwd2 is.
-constexpr int kPtRows = 32 * kPaWaves, kPtWin = 2048;
+constexpr int kPtRows = 32 * kPaWaves;
 
 // fa2_dma16 for a resource made right before it: its words come from v_readlane / v_readfirstlane, and a vector
 // memory instruction may read a scalar register that the VALU wrote only five wait states later. The compiler
@@ -668,13 +667,9 @@ __device__ __forceinline__ void pa_dma16(const u32x4& rsrc, uint32_t voff, uint3
       : "v"(voff), "s"(rsrc), "{m0}"(lds)
       : "memory");
 }
-// fdiv for divisors of 8 and more: its shift is past the low word
-__device__ __forceinline__ uint32_t pt_div(uint32_t n, FastDiv f) { return __umulhi(n, f.m) >> (f.s - 1); }
-
 template <int D>
 struct PtShared {
   uint16_t k[2 * kFaBKV * D], v[2 * kFaBKV * D];
-  int page[kPtWin];
   int again;
 };
 template <typename T, int D>
@@ -712,69 +707,56 @@ __device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, Pt
     const int lim1 = pa_uniform(min(pa_seen(it, min(rw0 + 31, rows - 1), a.f_g), kend));
     const int jw = pa_uniform(rw0 < rows && lim1 > kbeg ? (lim1 - 1 - kbeg) / kFaBKV : -1);  // the wave's last tile
 
-    // page numbers kbeg / page_size .. (kend - 1) / page_size, entry e at e % kPtWin
-    const int32_t* tab = a.s.table + it.b * a.s.table_stride;
-    const int e_last = pa_uniform((int)fdiv((uint32_t)(kend - 1), a.s.page_div));
-    constexpr int kHalf = kPtWin / 2;
-    int half = pa_uniform((int)fdiv((uint32_t)kbeg, a.s.page_div) / kHalf);  // the half that V's transfers have come to
-    auto fill = [&](int h) {
-      for (int e = h * kHalf + (int)threadIdx.x; e < (h + 1) * kHalf && e <= e_last; e += kPaThreads)
-        sh.page[e % kPtWin] = tab[e];
-    };
-    fill(half);
-    fill(half + 1);
-    __syncthreads();
-
     const uint16_t* Qr = (const uint16_t*)a.q + tok * a.qst + head * a.qsh;
     u32x4 qf[NS];
 #pragma unroll
     for (int s = 0; s < NS; ++s) qf[s] = my_r < rows ? ld16(Qr + s * 16 + hh * 8) : u32x4{0u, 0u, 0u, 0u};
 
-    // Byte offset of a lane inside a transfer: lane L writes physical chunk L % DC of row L / DC and so fetches
-    // the logical chunk that the swizzle maps there. (A wave's transfers start at rows that the swizzles do not
-    // tell apart.)
-    const int srow = w * RPI + lane / DC;
-    const uint32_t offk = (uint32_t)((lane / DC) * (int)a.kct * 2 + (((lane % DC) ^ fa2_kswz<D>(srow)) * 16));
-    const uint32_t offv = (uint32_t)((lane / DC) * (int)a.vct * 2 + (((lane % DC) ^ fa2_vswz<D>(srow)) * 16));
-    const uint32_t sK_lds = (uint32_t)(uintptr_t)(lds_void*)sh.k, sV_lds = (uint32_t)(uintptr_t)(lds_void*)sh.v;
-    // Lane i % NIW prepares transfer i of a tile, all transfers side by side: address and bytes of its keys.
-    // (Made by the scalar unit one transfer after another, 35 instructions each, they cost a third of the
-    // kernel's time.)
-    const int koff = kbeg + ((lane & (NIW - 1)) * kPaWaves + w) * RPI;
-    auto entry = [&](int j) { return pt_div((uint32_t)min(j * kFaBKV + koff, kend - 1), a.s.page_div); };
-    auto issue = [&](const uint16_t* base, uint32_t page_bytes, uint32_t slot_bytes, uint32_t off, int page, int j,
-                     uint32_t lds) {
-      const int key = j * kFaBKV + koff, left = min(kend - key, RPI);
-      const uint32_t slot = (uint32_t)key - pt_div((uint32_t)key, a.s.page_div) * (uint32_t)a.s.page_size;
-      const bool in = (uint32_t)page < (uint32_t)a.s.num_pages, any = left > 0;
-      bad |= any && !in;
-      const uint64_t at = (uint64_t)(uintptr_t)base + (uint64_t)(uint32_t)page * page_bytes + (uint64_t)slot * slot_bytes;
-      const uint32_t lo = (uint32_t)at, hi = (uint32_t)(at >> 32) & 0xffffu;
-      const uint32_t n = any && in ? (uint32_t)(left - 1) * slot_bytes + D * 2 : 0u;
+    // Byte offsets of a lane inside its wave's 16 keys: transfer i writes rows 16 w + i RPI .. of the tile, lane L
+    // physical chunk L % DC of row L / DC of them, and so fetches the logical chunk that the swizzle maps there.
+    uint32_t offk[NIW], offv[NIW];
 #pragma unroll
-      for (int i = 0; i < NIW; ++i) {
-        const u32x4 rs = {(uint32_t)__builtin_amdgcn_readlane((int)lo, i), (uint32_t)__builtin_amdgcn_readlane((int)hi, i),
-                          (uint32_t)__builtin_amdgcn_readlane((int)n, i), 0x00020000u};
-        pa_dma16(rs, off, lds + (i * kPaWaves + w) * 1024);
-      }
+    for (int i = 0; i < NIW; ++i) {
+      const int in16 = i * RPI + lane / DC;
+      offk[i] = (uint32_t)(in16 * (int)a.kct * 2 + (((lane % DC) ^ fa2_kswz<D>(in16)) * 16));
+      offv[i] = (uint32_t)(in16 * (int)a.vct * 2 + (((lane % DC) ^ fa2_vswz<D>(in16)) * 16));
+    }
+    const uint32_t sK_lds = (uint32_t)(uintptr_t)(lds_void*)sh.k, sV_lds = (uint32_t)(uintptr_t)(lds_void*)sh.v;
+    // Where the wave's keys of tile (j & ~63) + lane lie: address and bytes, all 64 tiles side by side. (Made for
+    // each tile and transfer by the scalar unit, 35 instructions each, this cost a third of the kernel's time.)
+    struct Where {
+      uint32_t lo, hi, n;
+    };
+    const int32_t* tab = a.s.table + it.b * a.s.table_stride;
+    auto find = [&](int j, const uint16_t* base, uint32_t page_bytes, uint32_t slot_bytes) {
+      const int key = kbeg + ((j & ~63) + lane) * kFaBKV + 16 * w, left = min(kend - key, 16);
+      const bool any = left > 0;
+      const uint32_t e = fdiv((uint32_t)min(key, kend - 1), a.s.page_div);
+      const uint32_t slot = (uint32_t)min(key, kend - 1) - e * (uint32_t)a.s.page_size;
+      const uint32_t page = (uint32_t)tab[e];
+      const bool in = page < (uint32_t)a.s.num_pages;
+      bad |= any && !in;
+      const uint64_t at = (uint64_t)(uintptr_t)base + (uint64_t)page * page_bytes + (uint64_t)slot * slot_bytes;
+      return Where{(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu,
+                   any && in ? (uint32_t)(left - 1) * slot_bytes + D * 2 : 0u};
+    };
+    auto issue = [&](const Where& x, int j, const uint32_t (&off)[NIW], uint32_t lds) {
+      const u32x4 rs = {(uint32_t)__builtin_amdgcn_readlane((int)x.lo, j & 63),
+                        (uint32_t)__builtin_amdgcn_readlane((int)x.hi, j & 63),
+                        (uint32_t)__builtin_amdgcn_readlane((int)x.n, j & 63), 0x00020000u};
+#pragma unroll
+      for (int i = 0; i < NIW; ++i) pa_dma16(rs, off[i], lds + (w * NIW + i) * 1024);
     };
     const uint16_t* Kb = (const uint16_t*)a.kc + it.hk * a.kch;
     const uint16_t* Vb = (const uint16_t*)a.vc + it.hk * a.vch;
-    int pk = sh.page[entry(0) % kPtWin], pv_ = pk;  // page numbers of the next K and V tile to be issued
+    Where wk, wv;
     auto issue_k = [&](int j, int stage) {
-      issue(Kb, (uint32_t)a.kcp * 2, (uint32_t)a.kct * 2, offk, pk, j, sK_lds + stage * TILE * 2);
-      pk = sh.page[entry(j + 1) % kPtWin];
+      if ((j & 63) == 0) wk = find(j, Kb, (uint32_t)a.kcp * 2, (uint32_t)a.kct * 2);
+      issue(wk, j, offk, sK_lds + stage * TILE * 2);
     };
     auto issue_v = [&](int j, int stage) {
-      issue(Vb, (uint32_t)a.vcp * 2, (uint32_t)a.vct * 2, offv, pv_, j, sV_lds + stage * TILE * 2);
-      const int h = pa_uniform((int)(pt_div((uint32_t)(kbeg + j * kFaBKV), a.s.page_div) / kHalf));
-      // every wave's V numbers of this half's tiles on come from this half or the next, every K number read so
-      // far too: the half behind can take the one after
-      if (h > half) {
-        half = h;
-        fill(half + 1);
-      }
-      pv_ = sh.page[entry(j + 1) % kPtWin];
+      if ((j & 63) == 0) wv = find(j, Vb, (uint32_t)a.vcp * 2, (uint32_t)a.vct * 2);
+      issue(wv, j, offv, sV_lds + stage * TILE * 2);
     };
 
     auto qk = [&](const uint16_t* ks, f32x16 (&s)[2]) {
@@ -863,7 +845,7 @@ __device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, Pt
     };
     // The DMA schedule and its waits are fa_fwd2's: tile t lives in stage t & 1; V_{j+1} is issued after
     // phase 1 of iteration j, K_{j+3} after phase 2, and a wait leaves the transfers issued later in flight.
-    // (page_of's LDS reads and fill's global loads come after them; the compiler's own waits cover those.)
+    // (The compiler's own waits cover find's global load.)
     auto barrier_after = [&](int later) {
       if (later >= 2) dma_barrier<2 * NIW>();
       else if (later == 1) dma_barrier<NIW>();
@@ -1037,12 +1019,12 @@ struct PaPlan {
   int64_t items[2], target[2], ws[2];  // ws: floats of a class's partials
   int64_t bytes() const { return (ws[0] + ws[1]) * (int64_t)sizeof(float); }
 };
-// fast: the MFMA kernels; paged8: pages of a multiple of 8 slots (pa_tiles)
+// fast: the MFMA kernels; pa_tiles needs pages of a multiple of 16 slots
 static PaPlan pa_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t page_size, int64_t width,
                       bool fast) {
   PaPlan p{};
   const int64_t keys = page_size * width, G = Hq / Hk, rows = T * G, seqs = std::min(B, T);
-  const bool tiles = fast && page_size % 8 == 0 && rows > kPaSplitRows;
+  const bool tiles = fast && page_size % 16 == 0 && rows > kPaSplitRows;
   p.bm0 = fast ? kPrRows : kPaRowTile;
   p.items[0] = (rows / p.bm0 + seqs) * Hk;
   if (tiles) {
@@ -1154,7 +1136,9 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
               host_aligned16(o);
   for (const int64_t x : {a.vcp, a.vch, a.vct, a.qst, a.qsh, a.ost, a.osh})
     if (x % 8 != 0) fast = false;
-  // pa_tiles addresses inside a page with 32 bits
+  // the fast kernels look a few steps past the last key with 32-bit positions; pa_tiles addresses inside a page
+  // with 32 bits
+  if (page_size * max_pages > INT_MAX - (1 << 16)) fast = false;
   for (const int64_t x : {a.kct, a.vct})
     if (x < D || x > (1 << 24) || x * page_size >= (int64_t)1 << 31) fast = false;
   for (const int64_t x : {a.kcp, a.vcp})
