@@ -38,6 +38,7 @@ struct PaArgs {
   void* o;
   PaClass c[2];    // few rows, many rows
   int split_rows;  // most rows (new tokens times group) of a sequence of class 0
+  FastDiv f_hq;
   int64_t qst, qsh, ost, osh;            // row and head strides (elements)
   int64_t kcp, kch, kct, vcp, vch, vct;  // cache: page, head, slot strides
   int Hq, Hk, G, D, Dp, vec;  // Dp: floats of a partial row, D rounded up to 4
@@ -68,12 +69,15 @@ struct PaItem {
   PaSeq seq;
 };
 
-__device__ __forceinline__ int pa_wave_scan(int v) {  // inclusive
-#pragma unroll
-  for (int o = 1; o < kWave; o <<= 1) {
-    const int x = __shfl_up(v, o, kWave);
-    if (lane_id() >= o) v += x;
-  }
+// Inclusive sum over the lanes: within rows of 16 lanes by row_shr, then each row's last lane to the rows after
+// it by row_bcast (six VALU instructions; __shfl_up goes through LDS six times).
+__device__ __forceinline__ int pa_wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
   return v;
 }
 
@@ -237,11 +241,11 @@ __device__ __forceinline__ float pa_inv(const PaSeq& q, bool sees, float l) {
 
 // Rows r_begin .. r_end - 1 of an item's tile over keys [lo, hi), one wave per row: results, or partials when
 // the keys are sliced.
-template <typename T, int BM, int CLS>
+template <typename T, int BM, int CLS, int NW = kPaWaves>
 __device__ void pa_one_by_one(const PaArgs& a, const PaItem& it, int r_begin, int r_end, int lo, int hi) {
   using S = typename T::S;
   const int lane = lane_id();
-  for (int r = r_begin + wave_id(); r < r_end; r += kPaWaves) {
+  for (int r = r_begin + wave_id(); r < r_end; r += NW) {
     const int tk = (int)fdiv((uint32_t)r, a.f_g);
     const int tok = it.seq.t0 + tk, h = it.hk * a.G + r - tk * a.G;
     const int seen = pa_seen(it, r, a.f_g);
@@ -282,11 +286,12 @@ __global__ __launch_bounds__(kPaThreads) void pa_general(const PaArgs a) {
 // (lane c: dims 4 c .. 4 c + 3 of each 64), then the groups' sums combine in group order. Four groups of one
 // wave for many rows; with few rows sixteen, so that 64 slices' partials are in flight at once. The grid is
 // bounded and walks the rows: in most calls with many rows nothing is sliced and it ends at once.
-template <typename T, int BM0, int BM1, int W>
+// JN: 64s of head_dim.
+template <typename T, int BM0, int BM1, int JN, int W>
 __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
   using S = typename T::S;
   constexpr int NG = 4 * W, NR = kPaWaves / W;  // groups of a row, rows of a block
-  __shared__ float so[kPaWaves * 4][260], sm[kPaWaves * 4], sl[kPaWaves * 4];
+  __shared__ float so[kPaWaves * 4][64 * JN + 4], sm[kPaWaves * 4], sl[kPaWaves * 4];
   const int lane = lane_id(), c = lane & 15;
   const int slot_in = pa_uniform(wave_id()) / W, g = (wave_id() % W) * 4 + lane / 16;
   const PaBatch x{pa_lane_seq(a.s, lane)};
@@ -298,23 +303,31 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
     return sliced;
   });
   if (!sliced) return;
+  // items of each class up to and with a lane's sequence
+  auto items = [&](const PaSeq& s, int (&n)[2], int (&upto)[2]) {
+    n[0] = pa_tiles_of<BM0, 0>(a, s) * a.Hk * pa_splits(s.len, chunk0);
+    n[1] = pa_tiles_of<BM1, 1>(a, s) * a.Hk * pa_splits(s.len, chunk1);
+    upto[0] = pa_wave_scan(n[0]);
+    upto[1] = pa_wave_scan(n[1]);
+  };
+  int n64[2], upto64[2];
+  items(x.q, n64, upto64);
   const int64_t total = (int64_t)a.s.T * a.Hq;
   for (int64_t block = blockIdx.x; block * NR < total; block += gridDim.x) {
     const int64_t row = block * NR + slot_in;
-    const int tok = (int)(row / a.Hq), h = (int)(row - (int64_t)tok * a.Hq);
+    const int tok = pa_uniform((int)fdiv((uint32_t)min(row, total - 1), a.f_hq)), h = (int)(row - (int64_t)tok * a.Hq);
     // the row's sequence, and the items of its class before it
     PaSeq q{0, 0, 0, false};
     int cls = 0, nsplit = 1;
     uint32_t first = 0, before[2] = {0, 0};
     if (row < total)
-      pa_each(a, x, [&](int, const PaSeq& s) {
+      pa_each(a, x, [&](int i, const PaSeq& s) {
         const uint64_t hit = __builtin_amdgcn_ballot_w64(tok >= s.t0 && tok < s.t0 + s.n);
-        const int n0 = pa_tiles_of<BM0, 0>(a, s) * a.Hk * pa_splits(s.len, chunk0);
-        const int n1 = pa_tiles_of<BM1, 1>(a, s) * a.Hk * pa_splits(s.len, chunk1);
-        const int i0 = pa_wave_scan(n0), i1 = pa_wave_scan(n1);
+        int n[2] = {n64[0], n64[1]}, upto[2] = {upto64[0], upto64[1]};
+        if (i > 0) items(s, n, upto);
         if (!hit) {
-          before[0] += (uint32_t)__builtin_amdgcn_readlane(i0, kWave - 1);
-          before[1] += (uint32_t)__builtin_amdgcn_readlane(i1, kWave - 1);
+          before[0] += (uint32_t)__builtin_amdgcn_readlane(upto[0], kWave - 1);
+          before[1] += (uint32_t)__builtin_amdgcn_readlane(upto[1], kWave - 1);
           return false;
         }
         const int l = __builtin_ctzll(hit);
@@ -324,23 +337,23 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
         q.overlong = __builtin_amdgcn_readlane((int)s.overlong, l) != 0;
         cls = q.n * a.G <= a.split_rows ? 0 : 1;
         nsplit = pa_splits(q.len, cls ? chunk1 : chunk0);
-        first = before[cls] + (uint32_t)__builtin_amdgcn_readlane(cls ? i1 - n1 : i0 - n0, l);
+        first = before[cls] + (uint32_t)__builtin_amdgcn_readlane(cls ? upto[1] - n[1] : upto[0] - n[0], l);
         return true;
       });
     const int bm = cls ? BM1 : BM0;
     const PaClass& cl = a.c[cls];
-    float m = -INFINITY, l = 0.f, acc[4][4];
+    float m = -INFINITY, l = 0.f, acc[JN][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < JN; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
     if (nsplit > 1) {
       const int tiles = (q.n * a.G + bm - 1) / bm;
-      const int hk = h / a.G, r = (tok - q.t0) * a.G + h % a.G;
+      const int hk = (int)fdiv((uint32_t)h, a.f_g), r = (tok - q.t0) * a.G + h - hk * a.G;
       const uint32_t it0 = first + (uint32_t)(tiles - 1 - r / bm) * a.Hk + hk;
       for (int sp = g; sp < nsplit; sp += 4 * NG) {
         float ms[4], ls[4];
-        f32x4 v[4][4];
+        f32x4 v[4][JN];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const uint32_t it = it0 + (uint32_t)(sp + u * NG) * tiles * a.Hk;
@@ -351,7 +364,7 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
           ms[u] = cl.stat[slot * 2];
           ls[u] = cl.stat[slot * 2 + 1];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < JN; ++j)
             if (64 * j + 4 * c < a.D) v[u][j] = *reinterpret_cast<const f32x4*>(cl.part + slot * a.Dp + 64 * j + 4 * c);
         }
 #pragma unroll
@@ -363,7 +376,7 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
           m = m_new;
           l = l * f0 + ls[u] * f1;
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; j < JN; ++j)
             if (64 * j + 4 * c < a.D)
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] * f0 + v[u][j][e] * f1;
@@ -373,7 +386,7 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
     const int me = slot_in * NG + g;
     __syncthreads();  // the block's last rows have been read
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < JN; ++j)
       if (64 * j + 4 * c < a.D)
         *reinterpret_cast<f32x4*>(&so[me][64 * j + 4 * c]) = f32x4{acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
     if (c == 0) {
@@ -432,14 +445,85 @@ struct PrVec<64> {
   typedef u32x2 type;
 };
 
-template <int D>
+template <int D, int NW>
 struct PrShared {
-  float so[kPaWaves][kPrRows][D + 4];
-  float st[kPaWaves][kPrRows][2];
+  float so[NW][kPrRows][D + 4];
+  float st[NW][kPrRows][2];
   int again;
 };
-template <typename T, int D, int PG>
-__device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrShared<D>& sh) {
+
+// The end of a few-row item: the waves' results (lane (i16, g) holds of row i16, in o[e][v], dim VW (4 g + v) + e)
+// merged and stored, or the rows computed again.
+template <typename T, int D, int NW>
+__device__ __forceinline__ void pr_finish(const PaArgs& a, const PaItem& it, PrShared<D, NW>& sh,
+                                          const f32x4 (&o)[D / 16], float m_run, float l_run, bool bad, int rows, int r0,
+                                          int kbeg, int kend) {
+  constexpr int VW = D / 16;
+  const int lane = lane_id(), w = wave_id(), i16 = lane & 15, g = lane >> 4;
+  l_run = pr_groups(l_run, OpAdd());
+  bad |= l_run != l_run;
+#pragma unroll
+  for (int e = 0; e < VW; ++e)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) bad |= o[e][v] != o[e][v];
+#pragma unroll
+  for (int v = 0; v < 4; ++v)
+#pragma unroll
+    for (int e = 0; e < VW; ++e) sh.so[w][i16][VW * (4 * g + v) + e] = o[e][v];
+  if (g == 0) {
+    sh.st[w][i16][0] = m_run;
+    sh.st[w][i16][1] = l_run;
+  }
+  __syncthreads();  // (the flag is cleared by now)
+  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) atomicOr(&sh.again, 1);
+  __syncthreads();
+  if (sh.again) {
+    pa_one_by_one<T, kPrRows, 0, NW>(a, it, r0, min(rows, r0 + kPrRows), kbeg, kend);
+    return;
+  }
+  const int q = threadIdx.x >> 4, c = threadIdx.x & 15;  // row of the tile, VW dims at c * VW
+  if (q >= kPrRows || r0 + q >= rows) return;
+  float mb = -INFINITY, l = 0.f, acc[VW];
+#pragma unroll
+  for (int x = 0; x < NW; ++x) mb = fmaxf(mb, sh.st[x][q][0]);
+#pragma unroll
+  for (int e = 0; e < VW; ++e) acc[e] = 0.f;
+#pragma unroll
+  for (int x = 0; x < NW; ++x) {
+    const float f = sh.st[x][q][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh.st[x][q][0] - mb);
+    l += sh.st[x][q][1] * f;
+#pragma unroll
+    for (int e = 0; e < VW; ++e) acc[e] += sh.so[x][q][c * VW + e] * f;
+  }
+  if (it.nsplit > 1) {
+    const int64_t slot = (int64_t)it.slot * kPrRows + q;
+    float* p = a.c[0].part + slot * a.Dp + c * VW;
+#pragma unroll
+    for (int e = 0; e < VW; e += 4) *reinterpret_cast<f32x4*>(p + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
+    if (c == 0) {
+      a.c[0].stat[slot * 2] = mb;
+      a.c[0].stat[slot * 2 + 1] = l;
+    }
+    return;
+  }
+  const float inv = pa_inv(it.seq, pa_seen(it, r0 + q, a.f_g) > 0, l);
+  const int tk = (int)fdiv((uint32_t)(r0 + q), a.f_g);
+  typename T::S* dst = (typename T::S*)a.o + (int64_t)(it.seq.t0 + tk) * a.ost +
+                       (int64_t)(it.hk * a.G + r0 + q - tk * a.G) * a.osh + c * VW;
+  if constexpr (T::kCode == AK_F32) {
+#pragma unroll
+    for (int e = 0; e < VW; e += 4)
+      *reinterpret_cast<f32x4*>(dst + e) = f32x4{acc[e] * inv, acc[e + 1] * inv, acc[e + 2] * inv, acc[e + 3] * inv};
+  } else {
+    typename PrVec<D>::type pk;
+#pragma unroll
+    for (int e = 0; e < VW / 2; ++e) pk[e] = fa2_pack<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    *reinterpret_cast<typename PrVec<D>::type*>(dst) = pk;
+  }
+}
+
+template <typename T, int D, int PG, int NW>
+__device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrShared<D, NW>& sh) {
   constexpr int NS = D / 32, VW = D / 16;
   constexpr int NK = PG == 8 ? 1 : 2, NV = PG == 8 ? 1 : 8;  // page numbers of a lane and step
   using VV = typename PrVec<D>::type;
@@ -563,7 +647,7 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
     }
   };
 
-  constexpr int kStride = kPaWaves * kPrKeys;
+  constexpr int kStride = NW * kPrKeys;
   int k0 = kbeg + pa_uniform(w) * kPrKeys;
   if (k0 < kend) {
     Step s0, s1;
@@ -586,61 +670,138 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
       k0 += kStride;
     }
   }
-  l_run = pr_groups(l_run, OpAdd());
-  bad |= l_run != l_run;
-#pragma unroll
-  for (int e = 0; e < VW; ++e)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) bad |= o[e][v] != o[e][v];
+  pr_finish<T, D, NW>(a, it, sh, o, m_run, l_run, bad, rows, r0, kbeg, kend);
+}
 
-  // Merge the waves: lane (i16, g) holds of row i16, in o[e][v], dim VW (4 g + v) + e.
+// The same in fp32 (v_mfma_f32_16x16x4, whose products and sums are fp32), 16 keys a step. A lane's K operand is
+// a quarter of one key's row: the contraction's order is free, so k index g of step s is dim g D / 4 + s and K
+// and Q load as whole vectors. S^T leaves lane group g with the scores of keys 4 g .. 4 g + 3, so step t of
+// O^T += V^T P^T takes keys 4 g + t: weight t as it stands, and the V rows of four consecutive keys.
+template <int D, int PG, int NW>
+__device__ __forceinline__ void pa_rows_f32_item(const PaArgs& a, uint32_t item, PrShared<D, NW>& sh) {
+  constexpr int NS = D / 4, VW = D / 16;
+  constexpr int kKeys = 16, NV = PG == 4 ? 1 : 4;
+  PaItem it;
+  if (!pa_find<kPrRows, 0>(a, item, it)) return;
+  if (threadIdx.x == 0) sh.again = 0;
+  const int lane = lane_id(), w = wave_id();
+  const int i16 = lane & 15, g = lane >> 4;
+  const float* Kb = (const float*)a.kc + it.hk * a.kch + g * NS;
+  const float* Vb = (const float*)a.vc + it.hk * a.vch + i16 * VW;
+  const int rows = it.seq.n * a.G, r0 = it.tile * kPrRows, r = r0 + i16;
+  const int lim = r < rows ? pa_seen(it, r, a.f_g) : 0;
+  f32x4 qf[NS / 4];
+  {
+    const int tk = (int)fdiv((uint32_t)min(r, rows - 1), a.f_g);
+    const float* q = (const float*)a.q + (int64_t)(it.seq.t0 + tk) * a.qst +
+                     (int64_t)(it.hk * a.G + min(r, rows - 1) - tk * a.G) * a.qsh + g * NS;
 #pragma unroll
-  for (int v = 0; v < 4; ++v)
-#pragma unroll
-    for (int e = 0; e < VW; ++e) sh.so[w][i16][VW * (4 * g + v) + e] = o[e][v];
-  if (g == 0) {
-    sh.st[w][i16][0] = m_run;
-    sh.st[w][i16][1] = l_run;
+    for (int s = 0; s < NS / 4; ++s)
+      qf[s] = r < rows ? *reinterpret_cast<const f32x4*>(q + 4 * s) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  __syncthreads();  // (the flag is cleared by now)
-  if (__builtin_amdgcn_ballot_w64(bad) && lane == 0) atomicOr(&sh.again, 1);
-  __syncthreads();
-  if (sh.again) {
-    pa_one_by_one<T, kPrRows, 0>(a, it, r0, min(rows, r0 + kPrRows), kbeg, kend);
-    return;
-  }
-  const int q = threadIdx.x >> 4, c = threadIdx.x & 15;  // row of the tile, VW dims at c * VW
-  if (r0 + q >= rows) return;
-  float mb = -INFINITY, l = 0.f, acc[VW];
+  const int rl = min(rows, r0 + kPrRows) - 1;
+  const int kbeg = pa_uniform(it.nsplit == 1 ? 0 : it.split * it.chunk);
+  const int kend = pa_uniform(min(pa_seen(it, rl, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk));
+  const int full = pa_uniform(pa_seen(it, r0, a.f_g));
+  struct Pages {
+    int k, v[NV];
+  };
+  const int32_t* tab = a.s.table + it.b * a.s.table_stride;
+  bool bad = false;
+  auto pages = [&](int k0, Pages& p) {
+    p.k = tab[fdiv((uint32_t)min(k0 + i16, kend - 1), a.s.page_div)];
 #pragma unroll
-  for (int x = 0; x < kPaWaves; ++x) mb = fmaxf(mb, sh.st[x][q][0]);
+    for (int x = 0; x < NV; ++x) p.v[x] = tab[fdiv((uint32_t)min(k0 + 4 * g + x, kend - 1), a.s.page_div)];
+  };
+  struct Step {
+    f32x4 k[NS / 4], v[4][VW / 4];
+  };
+  auto load = [&](int k0, const Pages& p, Step& st) {
+    {
+      const int key = min(k0 + i16, kend - 1);
+      const bool in = (uint32_t)p.k < a.s.num_pages;
+      bad |= !in;
+      const uint32_t slot = (uint32_t)key - fdiv((uint32_t)key, a.s.page_div) * a.s.page_size;
+      const float* src = Kb + (in ? p.k * a.kcp + slot * a.kct : 0);
 #pragma unroll
-  for (int e = 0; e < VW; ++e) acc[e] = 0.f;
-#pragma unroll
-  for (int x = 0; x < kPaWaves; ++x) {
-    const float f = sh.st[x][q][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sh.st[x][q][0] - mb);
-    l += sh.st[x][q][1] * f;
-#pragma unroll
-    for (int e = 0; e < VW; ++e) acc[e] += sh.so[x][q][c * VW + e] * f;
-  }
-  if (it.nsplit > 1) {
-    const int64_t slot = (int64_t)it.slot * kPrRows + q;
-    float* p = a.c[0].part + slot * a.Dp + c * VW;
-#pragma unroll
-    for (int e = 0; e < VW; e += 4) *reinterpret_cast<f32x4*>(p + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-    if (c == 0) {
-      a.c[0].stat[slot * 2] = mb;
-      a.c[0].stat[slot * 2 + 1] = l;
+      for (int s = 0; s < NS / 4; ++s)
+        st.k[s] = in ? *reinterpret_cast<const f32x4*>(src + 4 * s) : f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    return;
-  }
-  const float inv = pa_inv(it.seq, pa_seen(it, r0 + q, a.f_g) > 0, l);
-  const int tk = (int)fdiv((uint32_t)(r0 + q), a.f_g);
-  typename PrVec<D>::type pk;
 #pragma unroll
-  for (int e = 0; e < VW / 2; ++e) pk[e] = fa2_pack<T>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  *reinterpret_cast<VV*>((uint16_t*)a.o + (int64_t)(it.seq.t0 + tk) * a.ost +
-                         (int64_t)(it.hk * a.G + r0 + q - tk * a.G) * a.osh + c * VW) = pk;
+    for (int t = 0; t < 4; ++t) {
+      const int key = k0 + 4 * g + t, pg = p.v[PG == 4 ? 0 : t];
+      const bool in = (uint32_t)pg < a.s.num_pages && key < kend;
+      const uint32_t slot = (uint32_t)key - fdiv((uint32_t)key, a.s.page_div) * a.s.page_size;
+      const float* src = Vb + (in ? pg * a.vcp + slot * a.vct : 0);
+#pragma unroll
+      for (int e = 0; e < VW / 4; ++e)
+        st.v[t][e] = in ? *reinterpret_cast<const f32x4*>(src + 4 * e) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  f32x4 o[VW];
+#pragma unroll
+  for (int e = 0; e < VW; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.f;
+  auto compute = [&](int k0, const Step& st) {
+    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};  // even and odd steps: two chains
+#pragma unroll
+    for (int x = 0; x < NS; ++x)
+      s[x & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(st.k[x / 4][x % 4], qf[x / 4][x % 4], s[x & 1], 0, 0, 0);
+    f32x4 z = s[0] + s[1];
+    if (k0 + kKeys > full) {
+      const int left = min(lim, kend) - (k0 + 4 * g);
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        if (v >= left) z[v] = -INFINITY;
+    }
+    float mt = fa2_max(fa2_max(z[0], z[1]), fa2_max(z[2], z[3]));
+    mt = pr_groups(mt, PrMaximum());
+    const float m_new = fa2_max(m_run, mt * a.c_log2);
+    const float base = m_new == -INFINITY ? 0.f : m_new;
+    const float alpha = m_new == m_run ? 1.0f : __builtin_amdgcn_exp2f(m_run - base);
+    m_run = m_new;
+    float p[4], ps = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      p[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(z[v], a.c_log2, -base));
+      ps += p[v];
+    }
+    l_run = l_run * alpha + ps;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f)) {
+#pragma unroll
+      for (int e = 0; e < VW; ++e)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) o[e][v] *= alpha;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < VW; ++e) o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(st.v[t][e / 4][e % 4], p[t], o[e], 0, 0, 0);
+  };
+  constexpr int kStride = NW * kKeys;
+  int k0 = kbeg + pa_uniform(w) * kKeys;
+  if (k0 < kend) {
+    Step s0, s1;
+    Pages p0, p1;
+    pages(k0, p0);
+    if (k0 + kStride < kend) pages(k0 + kStride, p1);
+    load(k0, p0, s0);
+    while (true) {
+      const bool more1 = k0 + kStride < kend;
+      if (k0 + 2 * kStride < kend) pages(k0 + 2 * kStride, p0);
+      if (more1) load(k0 + kStride, p1, s1);
+      compute(k0, s0);
+      if (!more1) break;
+      k0 += kStride;
+      const bool more0 = k0 + kStride < kend;
+      if (k0 + 2 * kStride < kend) pages(k0 + 2 * kStride, p1);
+      if (more0) load(k0 + kStride, p0, s0);
+      compute(k0, s1);
+      if (!more0) break;
+      k0 += kStride;
+    }
+  }
+  pr_finish<TF32, D, NW>(a, it, sh, o, m_run, l_run, bad, rows, r0, kbeg, kend);
 }
 
 // Many rows per KV head: 128 rows a block, a wave owns 32, 64 keys a step through LDS. The pipeline of fa_fwd2
@@ -995,20 +1156,21 @@ __device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, Pt
     }
 }
 
-template <typename T, int D, int PG>
-__global__ __launch_bounds__(kPaThreads, 2) void pa_rows(const PaArgs a) {
-  __shared__ __attribute__((aligned(16))) PrShared<D> sh;
-  pa_rows_item<T, D, PG>(a, blockIdx.x, sh);
+template <typename T, int D, int PG, int NW>
+__global__ __launch_bounds__(NW* kWave, 2) void pa_rows(const PaArgs a) {
+  __shared__ __attribute__((aligned(16))) PrShared<D, NW> sh;
+  if constexpr (T::kCode == AK_F32) pa_rows_f32_item<D, PG == 8 ? 4 : 1, NW>(a, blockIdx.x, sh);
+  else pa_rows_item<T, D, PG, NW>(a, blockIdx.x, sh);
 }
 // Both classes in one launch: the blocks of the large tiles first.
 template <typename T, int D>
 __global__ __launch_bounds__(kPaThreads, 2) void pa_mixed(const PaArgs a) {
   __shared__ __attribute__((aligned(1024))) union {
     PtShared<D> t;
-    PrShared<D> r;
+    PrShared<D, kPaWaves> r;
   } sh;
   if (blockIdx.x < a.c[1].items) pa_tiles_item<T, D>(a, blockIdx.x, sh.t);
-  else pa_rows_item<T, D, 8>(a, blockIdx.x - a.c[1].items, sh.r);
+  else pa_rows_item<T, D, 8, kPaWaves>(a, blockIdx.x - a.c[1].items, sh.r);
 }
 
 // What a call launches: the most items of each class and their partials. Keys are sliced only where some
@@ -1020,11 +1182,11 @@ struct PaPlan {
   int64_t bytes() const { return (ws[0] + ws[1]) * (int64_t)sizeof(float); }
 };
 // fast: the MFMA kernels; pa_tiles needs pages of a multiple of 16 slots
-static PaPlan pa_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t page_size, int64_t width,
-                      bool fast) {
+static PaPlan pa_plan(int dtype, int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, int64_t page_size,
+                      int64_t width, bool fast) {
   PaPlan p{};
   const int64_t keys = page_size * width, G = Hq / Hk, rows = T * G, seqs = std::min(B, T);
-  const bool tiles = fast && page_size % 16 == 0 && rows > kPaSplitRows;
+  const bool tiles = fast && dtype != AK_F32 && page_size % 16 == 0 && rows > kPaSplitRows;
   p.bm0 = fast ? kPrRows : kPaRowTile;
   p.items[0] = (rows / p.bm0 + seqs) * Hk;
   if (tiles) {
@@ -1032,9 +1194,15 @@ static PaPlan pa_plan(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D, i
     p.items[1] = (rows / kPtRows + std::min(seqs, rows / (kPaSplitRows + 1))) * Hk;
   }
   if (keys > kPaMinSliced) {
-    p.target[0] = 1024;
+#ifndef PA_T1
+#define PA_T1 512
+#endif
+#ifndef PA_T0
+#define PA_T0 1536
+#endif
+    p.target[0] = PA_T0;
     // two tiles per CU at a time; four times that many are work enough unsliced
-    if (tiles && rows / kPtRows * Hk < 4 * 512) p.target[1] = 512;
+    if (tiles && rows / kPtRows * Hk < 4 * 512) p.target[1] = PA_T1;
   }
   const int64_t row = (D + 3) / 4 * 4 + 2;
   for (int c = 0; c < 2; ++c)
@@ -1056,29 +1224,45 @@ static void pa_set(PaArgs& a, const PaPlan& p, void* ws) {
   }
   a.split_rows = p.items[1] > 0 ? (int)kPaSplitRows : INT_MAX;
 }
-template <typename T, int BM0, int BM1>
+template <typename T, int BM0, int BM1, int JN>
 static void pa_launch_merge(const PaArgs& a, hipStream_t st) {
   if (a.c[0].target <= 0.f && a.c[1].target <= 0.f) return;
   const int64_t rows = (int64_t)a.s.T * a.Hq;
-  if (rows <= 4096) pa_merge<T, BM0, BM1, 4><<<dim3((unsigned)rows), kPaThreads, 0, st>>>(a);
-  else pa_merge<T, BM0, BM1, 1><<<dim3((unsigned)std::min<int64_t>(cdiv(rows, kPaWaves), 2048)), kPaThreads, 0, st>>>(a);
+  if (rows < 1024) pa_merge<T, BM0, BM1, JN, 4><<<dim3((unsigned)rows), kPaThreads, 0, st>>>(a);
+  else pa_merge<T, BM0, BM1, JN, 1><<<dim3((unsigned)std::min<int64_t>(cdiv(rows, kPaWaves), 2048)), kPaThreads, 0, st>>>(a);
 }
 template <typename T>
 static int launch_general(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
   pa_set(a, p, ws);
   pa_general<T><<<dim3((unsigned)p.items[0]), kPaThreads, 0, st>>>(a);
-  pa_launch_merge<T, kPaRowTile, kPaRowTile>(a, st);
+  pa_launch_merge<T, kPaRowTile, kPaRowTile, 4>(a, st);
   return record_launch();
+}
+// Blocks of eight waves where a batch has at most one per CU: each wave walks half as many keys.
+template <typename T, int D, int PG>
+static void launch_rows(const PaArgs& a, const PaPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)p.items[0]);
+  if (p.items[0] <= 256) pa_rows<T, D, PG, 8><<<grid, 8 * kWave, 0, st>>>(a);
+  else pa_rows<T, D, PG, kPaWaves><<<grid, kPaThreads, 0, st>>>(a);
 }
 template <typename T, int D>
 static int launch_fast(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
   pa_set(a, p, ws);
-  const dim3 grid((unsigned)(p.items[0] + p.items[1]));
-  if (p.items[1] > 0) pa_mixed<T, D><<<grid, kPaThreads, 0, st>>>(a);
-  else if (a.s.page_size % 8 == 0) pa_rows<T, D, 8><<<grid, kPaThreads, 0, st>>>(a);
-  else pa_rows<T, D, 1><<<grid, kPaThreads, 0, st>>>(a);
-  pa_launch_merge<T, kPrRows, kPtRows>(a, st);
+  if constexpr (T::kCode != AK_F32) {
+    if (p.items[1] > 0) {
+      pa_mixed<T, D><<<dim3((unsigned)(p.items[0] + p.items[1])), kPaThreads, 0, st>>>(a);
+      pa_launch_merge<T, kPrRows, kPtRows, D / 64>(a, st);
+      return record_launch();
+    }
+  }
+  if (a.s.page_size % 8 == 0) launch_rows<T, D, 8>(a, p, st);
+  else launch_rows<T, D, 1>(a, p, st);
+  pa_launch_merge<T, kPrRows, kPrRows, D / 64>(a, st);
   return record_launch();
+}
+template <typename T>
+static int launch_fast(const PaArgs& a, const PaPlan& p, void* ws, hipStream_t st) {
+  return a.D == 64 ? launch_fast<T, 64>(a, p, ws, st) : launch_fast<T, 128>(a, p, ws, st);
 }
 
 static bool pa_sizes_ok(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D) {
@@ -1097,9 +1281,8 @@ extern "C" int64_t ak_paged_attn_workspace_bytes(int dtype, int64_t T, int64_t B
   if (dtype != AK_F32 && dtype != AK_F16 && dtype != AK_BF16) return 0;
   if (!pa_sizes_ok(T, B, Hq, Hkv, D) || T == 0 || B == 0 || Hq == 0 || page_size <= 0 || max_pages < 0) return 0;
   if (page_size > INT_MAX || max_pages > INT_MAX) return 0;
-  const bool fast = dtype != AK_F32 && (D == 64 || D == 128);
-  return std::max(pa_plan(T, B, Hq, Hkv, D, page_size, max_pages, fast).bytes(),
-                  pa_plan(T, B, Hq, Hkv, D, page_size, max_pages, false).bytes());
+  return std::max(pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, D == 64 || D == 128).bytes(),
+                  pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, false).bytes());
 }
 
 extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o,
@@ -1128,14 +1311,14 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
   a.c_log2 = sm_scale * kFaLog2e;
   a.f_g = make_fastdiv((uint32_t)a.G);
   a.f_hk = make_fastdiv((uint32_t)a.Hk);
+  a.f_hq = make_fastdiv((uint32_t)a.Hq);
   a.s = make_paged(page_table, q_starts, kv_lens, T, B, num_pages, page_size, max_pages, table_stride);
   // K rows in 16-byte vectors
   const int vw = dtype == AK_F32 ? 4 : 8;
   a.vec = D % vw == 0 && host_aligned16(k_cache) && a.kcp % vw == 0 && a.kch % vw == 0 && a.kct % vw == 0;
-  bool fast = a.vec && dtype != AK_F32 && (D == 64 || D == 128) && host_aligned16(v_cache) && host_aligned16(q) &&
-              host_aligned16(o);
+  bool fast = a.vec && (D == 64 || D == 128) && host_aligned16(v_cache) && host_aligned16(q) && host_aligned16(o);
   for (const int64_t x : {a.vcp, a.vch, a.vct, a.qst, a.qsh, a.ost, a.osh})
-    if (x % 8 != 0) fast = false;
+    if (x % vw != 0) fast = false;
   // the fast kernels look a few steps past the last key with 32-bit positions; pa_tiles addresses inside a page
   // with 32 bits
   if (page_size * max_pages > INT_MAX - (1 << 16)) fast = false;
@@ -1143,11 +1326,8 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
     if (x < D || x > (1 << 24) || x * page_size >= (int64_t)1 << 31) fast = false;
   for (const int64_t x : {a.kcp, a.vcp})
     if (x < 0 || x >= (int64_t)1 << 31) fast = false;
-  const PaPlan p = pa_plan(T, B, Hq, Hkv, D, page_size, max_pages, fast);
-  if (fast) {
-    if (dtype == AK_F16)
-      return D == 64 ? launch_fast<TF16, 64>(a, p, workspace, stream) : launch_fast<TF16, 128>(a, p, workspace, stream);
-    return D == 64 ? launch_fast<TBF16, 64>(a, p, workspace, stream) : launch_fast<TBF16, 128>(a, p, workspace, stream);
-  }
-  AK_DISPATCH(dtype, T_, return launch_general<T_>(a, p, workspace, stream));
+  const PaPlan p = pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, fast);
+  AK_DISPATCH(dtype, T_, {
+    return fast ? launch_fast<T_>(a, p, workspace, stream) : launch_general<T_>(a, p, workspace, stream);
+  });
 }
