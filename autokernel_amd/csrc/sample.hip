@@ -13,12 +13,17 @@
 // token is the same on every run. A row of 2^20 weights stays below 2^62.
 //
 // One block of 16 waves per row:
-//   1. maximum (as an order-preserving integer key, its lowest index, NaN check)
-//   2. histogram of the row over kBins equal steps of log w, from the maximum down to 2^-44 (below, a weight
-//      adds nothing): counts, and masses unless top-k makes them needless
+//   1. the maximum
+//   2. a histogram of the row over kBins equal steps of log w, from the maximum down to 2^-44 (below, a weight
+//      adds nothing): of masses, or of counts while top-k is to be found
 //   3. the bins' running sums name the bin where a border lies. Where the bins down to it hold few enough
-//      elements they are gathered as (key, index) pairs and sorted in LDS, and every border falls out of one
-//      scan. Otherwise each border's own bin is gathered, cut into finer bins first while it holds too many.
+//      elements, these are gathered as (key, index) pairs and sorted in LDS, and the borders fall out of one
+//      scan. Otherwise the border's own bin is gathered, cut into finer ranges first while it holds too many.
+//      (A top-k border found that way becomes a bound on the row, and step 2 is done again with masses.)
+// What bounds it: the 64-bit weights of a whole row where no top-k spares them, about 28 instructions an
+// element. So everything else an element meets is one or two comparisons: a bin, or min-p, is a range of
+// floats, whose end is found once per row by trying 64 candidates at a time.
+#include <float.h>
 #include <limits.h>
 
 #include "ak_common.h"
@@ -27,10 +32,11 @@ namespace ak {
 
 constexpr int kSmThreads = 1024;
 constexpr int kSmWaves = kSmThreads / kWave;
-constexpr int kBins = 4096, kBinsPer = kBins / kSmThreads;
-constexpr int kList = 4096, kListPer = kList / kSmThreads;
-constexpr float kSpan = 44.0f;                // octaves of weight that the bins cover
-constexpr uint64_t kFixOne = 1ull << 42;      // weight 1
+constexpr int kPer = 4;                         // bins or list entries of a thread
+constexpr int kBins = kPer * kSmThreads, kList = kBins;
+constexpr int kRanked = 512;                    // lists up to this are ordered by counting, not by a sort network
+constexpr float kMaxTemperature = 1e30f;        // differences of floats up to the largest stay tellable
+constexpr float kSpan = 44.0f;                  // octaves of weight that the bins cover
 
 struct SampleArgs {
   const void* x;
@@ -44,12 +50,10 @@ struct SampleArgs {
 };
 
 struct SampleShared {
-  uint64_t mass[kBins];
-  uint32_t cnt[kBins];
-  uint64_t list[kList];
-  uint64_t red[kSmWaves];
-  uint64_t red2[kSmWaves];
-  uint64_t found[4];   // a border's element or bin, count and mass before it
+  uint64_t hist[kBins];
+  uint64_t list[kList];  // (the finer bins' histogram while a bin is cut up)
+  uint64_t red[kSmWaves], red2[kSmWaves];
+  uint64_t found[3];     // a border: its entry, the sum up to it, the sum before it
   uint32_t n;
 };
 
@@ -62,16 +66,18 @@ __device__ __forceinline__ float sm_val(uint32_t k) {
   return __uint_as_float(k ^ ((int32_t)k < 0 ? 0x80000000u : 0xffffffffu));
 }
 // (key, index) as one number whose falling order is the sorting order
-__device__ __forceinline__ uint64_t sm_pair(uint32_t key, int i) { return (uint64_t)key << 32 | (uint32_t)~i; }
+__device__ __forceinline__ uint64_t sm_pair(float x, int i) { return (uint64_t)sm_key(x) << 32 | (uint32_t)~i; }
 
 struct SampleRow {
-  double top, c;   // maximum; log2(e) / t
+  double top, c;     // maximum; log2(e) / t
   float topf, step;  // maximum; bins per unit of x
-  uint32_t low;    // smallest key that min-p keeps
+  float low;         // smallest value that counts (min-p, the bins' span, top-k); of its equals those up to
+  int low_last;      // index low_last
+  float min_p;
 };
 
-// 2^y for y <= 0: rounded to an integer n plus |f| <= 1/2, the Taylor polynomial of 2^f (its first term left
-// out is below 2.3e-13) and a shift of the exponent.
+// 2^y for y <= 0: rounded to an integer n plus |f| <= 1/2, the Taylor polynomial of 2^f (its first term
+// left out is below 2.3e-13) and a shift of the exponent.
 __device__ __forceinline__ double sm_exp2(double y) {
   const double n = __builtin_rint(y), f = y - n;
   double r = 7.0549116208011232e-09;
@@ -88,292 +94,283 @@ __device__ __forceinline__ double sm_exp2(double y) {
   return __builtin_ldexp(r, (int)n);
 }
 __device__ __forceinline__ double sm_weight(const SampleRow& r, float x) {
-  if (x == r.topf) return 1.0;
-  const double y = ((double)x - r.top) * r.c;
-  return y < -1000.0 ? 0.0 : sm_exp2(y);
+  return sm_exp2(((double)x - r.top) * r.c);
 }
-// weight in units of 2^-42, rounded to nearest: 2^10 has this unit as its last place
+// Weight in units of 2^-42, rounded to nearest: 2^10 has this unit as its last place. (x within the bins.)
 __device__ __forceinline__ uint64_t sm_fixed(const SampleRow& r, float x) {
-  return __builtin_bit_cast(uint64_t, sm_weight(r, x) + 1024.0) - 0x4090000000000000ull;
+  return __builtin_bit_cast(uint64_t, sm_exp2(((double)x - r.top) * r.c) + 1024.0) - 0x4090000000000000ull;
 }
-// Bin of x (falls with x), or -1: too light to count, or below min-p.
-__device__ __forceinline__ int sm_bin(const SampleRow& r, float x) {
-  if (x == r.topf) return 0;
-  const float f = (r.topf - x) * r.step;
-  return f < (float)kBins && sm_key(x) >= r.low ? (int)f : -1;
+// Bin of x <= topf: rises as x falls (each operation rounds monotonically). kBins and more: too light.
+__device__ __forceinline__ float sm_bin(const SampleRow& r, float x) { return (r.topf - x) * r.step; }
+
+// Smallest float of bin `last` or an earlier one with w >= min_p: 64 candidates a round, on every wave. (topf is one.)
+__device__ __forceinline__ float sm_first(const SampleRow& r, float last) {
+  uint32_t lo = 0, hi = sm_key(r.topf);  // in (lo, hi]; hi is one
+#pragma unroll 1
+  while (hi - lo > 1) {
+    const uint32_t step = max(1u, (hi - lo) / kWave);
+    const float v = sm_val(lo + step * (lane_id() + 1));
+    const bool past = step * (uint64_t)(lane_id() + 1) >= hi - lo;
+    const bool is = past || (sm_bin(r, v) < last + 1.0f && (r.min_p <= 0.f || sm_weight(r, v) >= (double)r.min_p));
+    const uint64_t m = __builtin_amdgcn_ballot_w64(is);  // candidates rise: all after the first
+    const int first = m ? __builtin_ctzll(m) : kWave;
+    if (first < kWave) hi = min(hi, lo + step * (first + 1));
+    lo += step * first;
+  }
+  return sm_val(hi);
 }
 
-// f(value, index) for every element of the row, 16-byte vectors between an unaligned head and tail. HEAVY: a
-// long f stands in the code once per 32-bit word of a vector, not once per element of it.
+// f(value, index) for every element of the row, 16-byte vectors between an unaligned head and tail, the next two
+// vectors in flight. +infinity counts as the largest finite float. HEAVY: a long f stands in the code once per
+// 32-bit word of a vector, not once per element of it.
 template <typename T, bool HEAVY, typename F>
 __device__ __forceinline__ void sm_each(const typename T::S* x, int V, F f) {
   constexpr int W = T::kVec;
+  const int tid = threadIdx.x;
   const int head = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(typename T::S));
   const int nv = (V - head) / W, tail = head + nv * W;
-  if ((int)threadIdx.x < head) f(T::to_f(x[threadIdx.x]), (int)threadIdx.x);
-  if ((int)threadIdx.x < V - tail) f(T::to_f(x[tail + threadIdx.x]), tail + (int)threadIdx.x);
-  // the next vector is in flight while one is worked on
-  u32x4 next = (int)threadIdx.x < nv ? ld16(x + head + (int64_t)threadIdx.x * W) : u32x4{0u, 0u, 0u, 0u};
+  const typename T::S* p = x + head;
+  auto load = [&](int i) { return ld16(p + (int64_t)min(i, nv - 1) * W); };
+  // head and tail: at most W - 1 elements each, on the first lanes of two waves
+  const int edge = tid < kWave ? (tid < head ? tid : -1) : (tid - kWave < V - tail ? tail + tid - kWave : -1);
+  if (tid < 2 * kWave && edge >= 0) f(fminf(T::to_f(x[edge]), FLT_MAX), edge);
+  if (nv == 0) return;
+  u32x4 next = load(tid), after = load(tid + kSmThreads);
 #pragma unroll 1
-  for (int i = threadIdx.x; i < nv; i += kSmThreads) {
+  for (int i = tid; i < nv; i += kSmThreads) {
     const u32x4 v = next;
-    if (i + kSmThreads < nv) next = ld16(x + head + (int64_t)(i + kSmThreads) * W);
+    next = after;
+    after = load(i + 2 * kSmThreads);
     if constexpr (HEAVY) {
       u32x4 w = v;
 #pragma unroll 1
       for (int q = 0; q < 4; ++q) {
 #pragma unroll
-        for (int e = 0; e < W / 4; ++e) f(T::lane_elem(w, e), head + i * W + q * (W / 4) + e);
+        for (int e = 0; e < W / 4; ++e) f(fminf(T::lane_elem(w, e), FLT_MAX), head + i * W + q * (W / 4) + e);
         w = u32x4{w[1], w[2], w[3], w[0]};
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < W; ++e) f(T::lane_elem(v, e), head + i * W + e);
+      for (int e = 0; e < W; ++e) f(fminf(T::lane_elem(v, e), FLT_MAX), head + i * W + e);
     }
   }
 }
 
 __device__ __forceinline__ uint64_t sm_wave_max(uint64_t v) {
-#pragma unroll
+#pragma unroll 1
   for (int o = kWave / 2; o > 0; o >>= 1) {
     const uint64_t w = __shfl_xor((unsigned long long)v, o, kWave);
     v = w > v ? w : v;
   }
   return v;
 }
-// Sum over the lower threads of the block (exclusive); total gets everyone's.
-__device__ __forceinline__ uint64_t sm_scan(uint64_t v, uint64_t* red, uint64_t& total) {
-  uint64_t s = v;
+__device__ __forceinline__ uint64_t sm_block_max(uint64_t v, uint64_t* red) {
+  v = sm_wave_max(v);
+  __syncthreads();
+  if (lane_id() == 0) red[wave_id()] = v;
+  __syncthreads();
+  return sm_wave_max(red[lane_id() % kSmWaves]);
+}
+
+// Running sums over kBins values, this thread's four: the sum before them, and up to each.
+struct SampleSums {
+  uint64_t before, upto[kPer];
+};
+__device__ __forceinline__ void sm_sums(SampleShared& sh, const uint64_t (&v)[kPer], SampleSums& s) {
+  uint64_t sum = 0;
 #pragma unroll
+  for (int i = 0; i < kPer; ++i) s.upto[i] = sum += v[i];
+  uint64_t run = sum;
+#pragma unroll 1
   for (int o = 1; o < kWave; o <<= 1) {
-    const uint64_t w = __shfl_up((unsigned long long)s, o, kWave);
-    if (lane_id() >= o) s += w;
+    const uint64_t w = __shfl_up((unsigned long long)run, o, kWave);
+    if (lane_id() >= o) run += w;
   }
   __syncthreads();
-  if (lane_id() == kWave - 1) red[wave_id()] = s;
+  if (lane_id() == kWave - 1) sh.red[wave_id()] = run;
   __syncthreads();
-  uint64_t before = 0;
-  total = 0;
+  s.before = run - sum;
+#pragma unroll 1
+  for (int i = 0; i < wave_id(); ++i) s.before += sh.red[i];
 #pragma unroll
-  for (int i = 0; i < kSmWaves; ++i) {
-    if (i < wave_id()) before += red[i];
-    total += red[i];
-  }
-  return before + s - v;
+  for (int i = 0; i < kPer; ++i) s.upto[i] += s.before;
 }
-
-// Falling order of list[0 .. n), padded with zeros to a power of two.
-__device__ __forceinline__ void sm_sort(SampleShared& sh, int n) {
-  int n2 = 1;
-  while (n2 < n) n2 <<= 1;
-  for (int i = n + threadIdx.x; i < n2; i += kSmThreads) sh.list[i] = 0;
-  for (int k = 2; k <= n2; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < n2 / 2; i += kSmThreads) {
-        const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const uint64_t p = sh.list[a], q = sh.list[b];
-        if ((p < q) == ((a & k) == 0)) {
-          sh.list[a] = q;
-          sh.list[b] = p;
-        }
-      }
-    }
-  __syncthreads();
-}
-
-enum SampleRule { kByCount, kReaches, kPasses };
-// Whether a running (count, mass) has arrived at the border.
-__device__ __forceinline__ bool sm_there(SampleRule rule, double target, uint64_t cnt, uint64_t mass) {
-  return rule == kByCount ? (double)cnt >= target : rule == kReaches ? (double)mass >= target : (double)mass > target;
-}
-
-// The bins' running sums, this thread's part: bins kBinsPer * tid ...
-struct SampleBins {
-  uint32_t cnt[kBinsPer + 1];
-  uint64_t mass[kBinsPer + 1];
-  uint64_t all_cnt, all_mass;
+// The first of the values whose running sum, with `base` before them all, reaches the target.
+struct SampleBorder {
+  int at;
+  uint64_t upto, before;
 };
-__device__ __forceinline__ void sm_sum_bins(SampleShared& sh, SampleBins& b) {
-  uint64_t c = 0, m = 0;
-#pragma unroll
-  for (int i = 0; i < kBinsPer; ++i) {
-    c += sh.cnt[threadIdx.x * kBinsPer + i];
-    m += sh.mass[threadIdx.x * kBinsPer + i];
-  }
-  b.cnt[0] = (uint32_t)sm_scan(c, sh.red, b.all_cnt);
-  b.mass[0] = sm_scan(m, sh.red2, b.all_mass);
-#pragma unroll
-  for (int i = 0; i < kBinsPer; ++i) {
-    b.cnt[i + 1] = b.cnt[i] + sh.cnt[threadIdx.x * kBinsPer + i];
-    b.mass[i + 1] = b.mass[i] + sh.mass[threadIdx.x * kBinsPer + i];
-  }
-}
-// Bin of the border and the count and mass before it (the last bin if rounding puts the border past it).
-struct SampleBin {
-  int bin;
-  uint32_t n;  // its elements
-  uint64_t cnt, mass;
-};
-__device__ __forceinline__ SampleBin sm_find_bin(SampleShared& sh, const SampleBins& b, SampleRule rule, double target) {
+__device__ __forceinline__ SampleBorder sm_find(SampleShared& sh, const SampleSums& s, uint64_t base, uint64_t target) {
   __syncthreads();
+  if (base + s.before < target && base + s.upto[kPer - 1] >= target) {
+    int i = 0;
+    uint64_t upto = s.upto[0], before = s.before;
 #pragma unroll
-  for (int i = 0; i < kBinsPer; ++i)
-    if (!sm_there(rule, target, b.cnt[i], b.mass[i]) && sm_there(rule, target, b.cnt[i + 1], b.mass[i + 1])) {
-      sh.found[0] = threadIdx.x * kBinsPer + i;
-      sh.found[1] = b.cnt[i];
-      sh.found[2] = b.mass[i];
-      sh.found[3] = b.cnt[i + 1] - b.cnt[i];
-    }
+    for (int j = 1; j < kPer; ++j)
+      if (base + upto < target) i = j, before = upto, upto = s.upto[j];
+    sh.found[0] = threadIdx.x * kPer + i;
+    sh.found[1] = base + upto;
+    sh.found[2] = base + before;
+  }
   __syncthreads();
-  return SampleBin{(int)sh.found[0], (uint32_t)sh.found[3], sh.found[1], sh.found[2]};
+  return SampleBorder{(int)sh.found[0], sh.found[1], sh.found[2]};
 }
 
-__device__ __forceinline__ void sm_clear_bins(SampleShared& sh) {
+// The running sum up to value `at`.
+__device__ __forceinline__ uint64_t sm_last(SampleShared& sh, const SampleSums& s, int at) {
   __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kSmThreads) {
-    sh.cnt[i] = 0;
-    sh.mass[i] = 0;
-  }
+  if ((int)threadIdx.x == at / kPer) sh.found[1] = at % kPer < 2 ? s.upto[at & 1] : s.upto[2 + (at & 1)];
   __syncthreads();
+  return sh.found[1];
 }
-
-// Running sums over the sorted list (this thread's entries kListPer * tid ..), starting from (cnt, mass).
-struct SampleList {
-  uint64_t mass[kListPer + 1];
-  uint32_t cnt0;
-  int n;
-};
-__device__ __forceinline__ void sm_sum_list(SampleShared& sh, const SampleRow& r, int n, uint64_t cnt, uint64_t mass,
-                                            SampleList& l) {
-  uint64_t w[kListPer], s = 0, total;
-#pragma unroll
-  for (int i = 0; i < kListPer; ++i) {
-    const int e = threadIdx.x * kListPer + i;
-    w[i] = e < n ? sm_fixed(r, sm_val((uint32_t)(sh.list[e] >> 32))) : 0;
-    s += w[i];
-  }
-  l.mass[0] = mass + sm_scan(s, sh.red, total);
-#pragma unroll
-  for (int i = 0; i < kListPer; ++i) l.mass[i + 1] = l.mass[i] + w[i];
-  l.cnt0 = (uint32_t)cnt;
-  l.n = n;
-}
-// The element at the border: index, and the mass up to and with it.
-struct SampleHit {
-  int index;
-  uint64_t mass;
-};
-__device__ __forceinline__ SampleHit sm_find_list(SampleShared& sh, const SampleList& l, SampleRule rule, double target) {
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kListPer; ++i) {
-    const int e = threadIdx.x * kListPer + i;
-    if (e < l.n && !sm_there(rule, target, l.cnt0 + e, l.mass[i]) &&
-        sm_there(rule, target, l.cnt0 + e + 1, l.mass[i + 1])) {
-      sh.found[0] = (uint32_t)~(uint32_t)sh.list[e];
-      sh.found[1] = l.mass[i + 1];
-    }
-  }
-  __syncthreads();
-  return SampleHit{(int)sh.found[0], sh.found[1]};
-}
-
-template <typename T>
-__device__ __forceinline__ void sm_gather(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V, int b0,
-                                          int b1, uint64_t lo, uint64_t hi) {
+// About how many elements the bins up to `at` hold: counted, or their masses over the weight in a bin's middle.
+__device__ __forceinline__ uint32_t sm_upto(SampleShared& sh, const SampleSums& s, int at, bool counts) {
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
-  sm_each<T, true>(x, V, [&](float v, int i) {
-    const int b = sm_bin(r, v);
-    if (b < b0 || b > b1) return;
-    const uint64_t e = sm_pair(sm_key(v), i);
-    if (e < lo || e > hi) return;
-    const uint32_t at = atomicAdd(&sh.n, 1u);
-    if (at < kList) sh.list[at] = e;
+  float n = 0.f;
+  uint64_t before = s.before;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int b = threadIdx.x * kPer + i;
+    const float in = (float)(s.upto[i] - before);
+    if (b <= at) n += counts ? in : in * __builtin_amdgcn_exp2f(((float)b + 0.5f) * (kSpan / kBins) - 42.0f);
+    before = s.upto[i];
+  }
+  n = wave_sum(n);
+  if (lane_id() == 0) atomicAdd(&sh.n, (uint32_t)(n + 0.5f));
+  __syncthreads();
+  return sh.n;
+}
+
+// What an element adds: 1, or its weight.
+template <typename T>
+__device__ __forceinline__ void sm_histogram(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V,
+                                             bool counts, SampleSums& s) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kSmThreads) sh.hist[i] = 0;
+  __syncthreads();
+  auto add = [&](float v, uint64_t w) {
+    atomicAdd((unsigned long long*)&sh.hist[(int)sm_bin(r, v)], (unsigned long long)w);
+  };
+  if (counts) {
+    sm_each<T, true>(x, V, [&](float v, int) {
+      if (v >= r.low) add(v, 1);
+    });
+  } else {
+    sm_each<T, true>(x, V, [&](float v, int i) {
+      if (v > r.low || (v == r.low && i <= r.low_last)) add(v, sm_fixed(r, v));
+    });
+  }
+  __syncthreads();
+  uint64_t v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) v[i] = sh.hist[threadIdx.x * kPer + i];
+  sm_sums(sh, v, s);
+}
+
+// Pairs in [lo, hi] of the row, into the list. sh.n: how many there are, which may be more than it holds.
+template <typename T>
+__device__ __forceinline__ void sm_gather(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V, uint64_t lo,
+                                          uint64_t hi) {
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  const float vlo = sm_val((uint32_t)(lo >> 32)), vhi = sm_val((uint32_t)(hi >> 32));
+  sm_each<T, false>(x, V, [&](float v, int i) {
+    if (v >= vlo && v <= vhi) {
+      const uint64_t e = sm_pair(v, i);
+      if (e >= lo && e <= hi) {
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < kList) sh.list[at] = e;
+      }
+    }
   });
   __syncthreads();
 }
 
-// A bin of more than kList elements is cut into kBins equal ranges of (key, index) until the border's range
-// [lo, hi] is small enough; `at` becomes that range.
-template <typename T>
-__device__ __forceinline__ void sm_narrow(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V,
-                                          SampleBin& at, SampleRule rule, double target, uint64_t& lo, uint64_t& hi) {
-#pragma unroll 1
-  while (at.n > kList) {
-    // the range that the elements really take
-    uint64_t a = 0, z = 0;  // largest, and largest complement
-    sm_each<T, true>(x, V, [&](float v, int i) {
-      if (sm_bin(r, v) != at.bin) return;
-      const uint64_t e = sm_pair(sm_key(v), i);
-      if (e < lo || e > hi) return;
-      a = e > a ? e : a;
-      z = ~e > z ? ~e : z;
-    });
-    a = sm_wave_max(a);
-    z = sm_wave_max(z);
+// The list in falling order, and its running sums (of ones, or of weights).
+__device__ __forceinline__ void sm_order(SampleShared& sh, const SampleRow& r, int n, bool counts, SampleSums& s) {
+  if (n <= kRanked) {
+    // an entry's place is the number of larger ones
+    const int tid = threadIdx.x;
+    const uint64_t me = tid < n ? sh.list[tid] : 0;
+    int place = 0;
+    if (tid < (n + kWave - 1) / kWave * kWave)
+#pragma unroll 4
+      for (int i = 0; i < n; ++i) place += sh.list[i] > me;
     __syncthreads();
-    if (lane_id() == 0) {
-      sh.red[wave_id()] = a;
-      sh.red2[wave_id()] = z;
-    }
-    __syncthreads();
-    for (int i = 0; i < kSmWaves; ++i) {
-      a = sh.red[i] > a ? sh.red[i] : a;
-      z = sh.red2[i] > z ? sh.red2[i] : z;
-    }
-    hi = a;
-    lo = ~z;
-    int shift = 0;
-    while (((hi - lo) >> shift) >= kBins) ++shift;
-    sm_clear_bins(sh);
-    sm_each<T, true>(x, V, [&](float v, int i) {
-      if (sm_bin(r, v) != at.bin) return;
-      const uint64_t e = sm_pair(sm_key(v), i);
-      if (e < lo || e > hi) return;
-      const int q = (int)((hi - e) >> shift);
-      atomicAdd(&sh.cnt[q], 1u);
-      atomicAdd((unsigned long long*)&sh.mass[q], (unsigned long long)sm_fixed(r, v));
-    });
-    __syncthreads();
-    SampleBins b;
-    sm_sum_bins(sh, b);
-    // the border counts from the row's start
-#pragma unroll
-    for (int i = 0; i <= kBinsPer; ++i) {
-      b.cnt[i] += (uint32_t)at.cnt;
-      b.mass[i] += at.mass;
-    }
-    const SampleBin in = sm_find_bin(sh, b, rule, target);
-    const uint64_t width = (1ull << shift) - 1;
-    hi -= (uint64_t)in.bin << shift;
-    if (hi >= width && hi - width > lo) lo = hi - width;
-    at.n = in.n;
-    at.cnt = in.cnt;
-    at.mass = in.mass;
-  }
-}
-
-template <typename T>
-__device__ __forceinline__ void sm_histogram(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V,
-                                             bool masses) {
-  sm_clear_bins(sh);
-  if (masses) {
-    sm_each<T, true>(x, V, [&](float v, int) {
-      const int b = sm_bin(r, v);
-      if (b < 0) return;
-      atomicAdd(&sh.cnt[b], 1u);
-      atomicAdd((unsigned long long*)&sh.mass[b], (unsigned long long)sm_fixed(r, v));
-    });
+    if (tid < n) sh.list[place] = me;
   } else {
-    sm_each<T, false>(x, V, [&](float v, int) {
-      const int b = sm_bin(r, v);
-      if (b >= 0) atomicAdd(&sh.cnt[b], 1u);
-    });
+    int n2 = kRanked;
+    while (n2 < n) n2 <<= 1;
+    for (int i = n + threadIdx.x; i < n2; i += kSmThreads) sh.list[i] = 0;
+#pragma unroll 1
+    for (int k = 2; k <= n2; k <<= 1)
+#pragma unroll 1
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        __syncthreads();
+#pragma unroll 1
+        for (int i = threadIdx.x; i < n2 / 2; i += kSmThreads) {
+          const int a = 2 * i - (i & (j - 1)), b = a + j;
+          const uint64_t p = sh.list[a], q = sh.list[b];
+          if ((p < q) == ((a & k) == 0)) {
+            sh.list[a] = q;
+            sh.list[b] = p;
+          }
+        }
+      }
   }
   __syncthreads();
+  uint64_t v[kPer];
+#pragma unroll 1
+  for (int i = 0; i < kPer; ++i) {
+    const int e = threadIdx.x * kPer + i;
+    const uint64_t w = e >= n ? 0 : counts ? 1 : sm_fixed(r, sm_val((uint32_t)(sh.list[e] >> 32)));
+    v[0] = i == 0 ? w : v[0], v[1] = i == 1 ? w : v[1], v[2] = i == 2 ? w : v[2], v[3] = i == 3 ? w : v[3];
+  }
+  sm_sums(sh, v, s);
+}
+
+// Cuts the pairs [lo, hi], `before` being the sum of the larger ones, to a range around the border that fits the
+// list: a histogram over kBins equal ranges of pairs, as often as it takes. Returns the elements in it, about.
+template <typename T>
+__device__ __forceinline__ void sm_narrow(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V, bool counts,
+                                          uint64_t target, uint64_t& lo, uint64_t& hi, uint64_t& before) {
+  // the range that the elements really take
+  uint64_t a = 0, z = 0;  // largest, and largest complement
+  const float vlo = sm_val((uint32_t)(lo >> 32)), vhi = sm_val((uint32_t)(hi >> 32));
+  sm_each<T, true>(x, V, [&](float v, int i) {
+    if (!(v >= vlo && v <= vhi)) return;
+    const uint64_t e = sm_pair(v, i);
+    if (e < lo || e > hi) return;
+    a = e > a ? e : a;
+    z = ~e > z ? ~e : z;
+  });
+  hi = sm_block_max(a, sh.red);
+  lo = ~sm_block_max(z, sh.red2);
+  int shift = 0;
+  while (((hi - lo) >> shift) >= kBins) ++shift;
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kSmThreads) sh.list[i] = 0;
+  __syncthreads();
+  sm_each<T, true>(x, V, [&](float v, int i) {
+    if (!(v >= vlo && v <= vhi)) return;
+    const uint64_t e = sm_pair(v, i);
+    if (e < lo || e > hi) return;
+    atomicAdd((unsigned long long*)&sh.list[(hi - e) >> shift], (unsigned long long)(counts ? 1 : sm_fixed(r, v)));
+  });
+  __syncthreads();
+  uint64_t v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) v[i] = sh.list[threadIdx.x * kPer + i];
+  SampleSums s;
+  sm_sums(sh, v, s);
+  const SampleBorder in = sm_find(sh, s, before, target);
+  const uint64_t width = (1ull << shift) - 1;
+  hi -= (uint64_t)in.at << shift;
+  if (hi >= width && hi - width > lo) lo = hi - width;
+  before = in.before;
 }
 
 template <typename T>
@@ -384,110 +381,108 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
   const S* x = (const S*)a.x + row * a.stride;
   const int V = a.V;
   const float t = a.tp ? a.tp[row] : a.t, top_p = a.pp ? a.pp[row] : a.p;
-  float min_p = a.mp ? a.mp[row] : a.m;
   const int top_k = a.kp ? a.kp[row] : a.k;
-  float uf = a.u[row];
-  uf = uf >= 0.f ? fminf(uf, 1.0f - 0x1p-24f) : 0.f;
-  const double u = uf;
-
-  // 1. maximum
-  uint64_t best = 0;
-  bool nan = false;
-  sm_each<T, false>(x, V, [&](float v, int i) {
-    nan |= v != v;
-    const uint64_t e = sm_pair(sm_key(v), i);
-    best = e > best ? e : best;
-  });
-  best = sm_wave_max(best);
-  const bool wnan = __builtin_amdgcn_ballot_w64(nan) != 0;
-  if (lane_id() == 0) {
-    sh.red[wave_id()] = best;
-    sh.red2[wave_id()] = wnan;
-  }
-  __syncthreads();
-  for (int i = 0; i < kSmWaves; ++i) {
-    best = sh.red[i] > best ? sh.red[i] : best;
-    nan |= sh.red2[i] != 0;
-  }
-  __syncthreads();
   SampleRow r;
-  r.topf = sm_val((uint32_t)(best >> 32));
+  r.min_p = a.mp ? a.mp[row] : a.m;
+  float u = a.u[row];
+  u = u >= 0.f ? fminf(u, 1.0f - 0x1p-24f) : 0.f;
+
+  // 1. maximum (v_maximum hands a NaN on, fminf above would lose it: the raw values)
+  float top;
+  {
+    float m = -INFINITY;
+    const int head = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(S));
+    const int nv = (V - head) / T::kVec, tail = head + nv * T::kVec;
+    for (int i = threadIdx.x; i < head; i += kSmThreads) m = __builtin_elementwise_maximum(m, T::to_f(x[i]));
+    for (int i = tail + threadIdx.x; i < V; i += kSmThreads) m = __builtin_elementwise_maximum(m, T::to_f(x[i]));
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nv; i += kSmThreads) {
+      const u32x4 v = ld16(x + head + (int64_t)i * T::kVec);
+#pragma unroll
+      for (int e = 0; e < T::kVec; ++e) m = __builtin_elementwise_maximum(m, T::lane_elem(v, e));
+    }
+    const uint64_t nan = __builtin_amdgcn_ballot_w64(m != m) ? 1 : 0;
+    const uint64_t best = (uint64_t)sm_key(m) << 1 | nan;
+    const uint64_t all = sm_block_max((nan << 40) | best, sh.red);
+    top = all >> 40 ? __builtin_nanf("") : sm_val((uint32_t)(all >> 1));
+  }
   // a NaN, nothing to draw, or settings that are no numbers
-  const bool none = nan || r.topf == -INFINITY || !(t >= 0.f && t < INFINITY) || top_p != top_p || min_p != min_p;
-  if (none || t == 0.f) {
-    if (threadIdx.x == 0) a.out[row] = none ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
+  if (!(top > -INFINITY) || !(t >= 0.f && t <= kMaxTemperature) || top_p != top_p || r.min_p != r.min_p) {
+    if (threadIdx.x == 0) a.out[row] = -1;
+    return;
+  }
+  r.topf = fminf(top, FLT_MAX);
+  if (t == 0.f) {  // the maximum's lowest index
+    uint64_t first = 0;
+    sm_each<T, true>(x, V, [&](float v, int i) {
+      if (v == r.topf) first = (uint32_t)~i > first ? (uint32_t)~i : first;
+    });
+    first = sm_block_max(first, sh.red);
+    if (threadIdx.x == 0) a.out[row] = (int64_t)(uint32_t)~(uint32_t)first;
     return;
   }
   r.top = r.topf;
   r.c = 1.4426950408889634 / (double)t;
-  r.step = (float)(r.c * (kBins / (double)kSpan));
-  r.low = 0;
-  if (min_p > 0.f) {
-    // smallest key of weight >= min_p, 64 candidates a step (weights rise with the key)
-    min_p = fminf(min_p, 1.0f);
-    uint32_t lo = 0, hi = (uint32_t)(best >> 32);  // the border is in (lo, hi], hi is kept
-    while (hi - lo > 1) {
-      const uint32_t step = max(1u, (hi - lo) / kWave);
-      const uint32_t at = lo + step * (lane_id() + 1);
-      const bool in = step * (uint64_t)(lane_id() + 1) < hi - lo;
-      const float v = sm_val(at);
-      const bool keep = !in || (v == v && sm_weight(r, v) >= (double)min_p);
-      const uint64_t m = __builtin_amdgcn_ballot_w64(keep);
-      const int first = m ? __builtin_ctzll(m) : kWave;  // candidates rise: the first that is kept
-      const uint32_t nlo = lo + step * first;
-      if (first < kWave) hi = min(hi, lo + step * (first + 1));
-      lo = nlo;
-    }
-    r.low = hi;
-  }
+  r.step = (float)fmin(r.c * (kBins / (double)kSpan), 1e30);
+  r.min_p = fminf(r.min_p, 1.0f);
+  r.low = sm_first(r, kBins - 1);
+  r.low_last = INT_MAX;
 
-  // 2. histogram: with top-k the counts alone, unless the first top_k elements are more than a list holds
-  SampleBins b;
-  const bool has_k = top_k > 0 && top_k < V, has_p = top_p < 1.0f;
-  bool cuts = false;  // top-k cuts something off
+  // 2, 3. the borders, one after another: top-k (while it is looked for, elements count 1 each), top-p, the
+  // token. A list that starts at the row's maximum holds the later borders too.
+  bool counts = top_k > 0 && top_k < V, listed = false;
+  SampleSums s;  // of the bins, or of the list
+  uint64_t z = 0;
+  int token = -1;
 #pragma unroll 1
-  for (bool masses = !has_k;; masses = true) {
-    sm_histogram<T>(sh, r, x, V, masses);
-    sm_sum_bins(sh, b);
-    cuts = has_k && (uint64_t)top_k < b.all_cnt;
-    if (masses) break;
-    uint64_t upto = b.all_cnt;
-    if (cuts) {
-      const SampleBin kb = sm_find_bin(sh, b, kByCount, top_k);
-      upto = kb.cnt + kb.n;
+  for (int step = counts ? 0 : 1; step < 3; ++step) {
+    if (!listed && (step < 2 || z == 0)) {
+      sm_histogram<T>(sh, r, x, V, counts, s);
+      z = sm_last(sh, s, kBins - 1);  // everything that is left
     }
-    if (upto <= kList) break;
-  }
-
-  // 3. the borders, one after another: top-k, top-p, the token. A list that starts at the row's maximum holds
-  // the later borders too.
-  double z = (double)b.all_mass;  // mass up to the last border
-  bool listed = false;
-  SampleList l;
-  SampleHit hit;
-#pragma unroll 1
-  for (int step = 0; step < 3; ++step) {
-    if (step == 0 ? !has_k : step == 1 ? !has_p : false) continue;
-    const SampleRule rule = step == 0 ? kByCount : step == 1 ? kReaches : kPasses;
-    // (a row with fewer elements than top_k ends at its last one)
-    const double target = step == 0 ? fmin((double)top_k, (double)b.all_cnt)
-                                    : step == 1 ? fmax((double)top_p * z, 1.0) : u * z;
+    if (step == 1 && !(top_p < 1.0f)) continue;
+    const uint64_t target = step == 0   ? min((uint64_t)top_k, z)  // a row with fewer elements ends at its last one
+                            : step == 1 ? max((uint64_t)__builtin_ceil((double)top_p * (double)z), (uint64_t)1)
+                                        : (uint64_t)((double)u * (double)z) + 1;
+    SampleBorder at = sm_find(sh, s, 0, target);
     if (!listed) {
-      SampleBin at = sm_find_bin(sh, b, rule, target);
-      uint64_t lo = 0, hi = ~0ull;
-      const int last = at.bin;
-      listed = at.cnt + at.n <= kList;
-      if (listed) at = SampleBin{0, (uint32_t)(at.cnt + at.n), 0, 0};
-      else sm_narrow<T>(sh, r, x, V, at, rule, target, lo, hi);
-      sm_gather<T>(sh, r, x, V, at.bin, last, lo, hi);
-      const int n = min((int)sh.n, kList);
-      sm_sort(sh, n);
-      sm_sum_list(sh, r, n, at.cnt, at.mass, l);
+      uint64_t lo = sm_pair(sm_first(r, (float)at.at), INT_MAX), hi = sm_pair(r.topf, 0), before = 0;
+      const uint64_t least = sm_pair(r.low, r.low_last);
+      if (lo < least) lo = least;
+      if (sm_upto(sh, s, at.at, counts) <= kList) {
+        sm_gather<T>(sh, r, x, V, lo, hi);
+        listed = sh.n <= kList;
+      }
+      if (!listed) {
+        if (at.at > 0) hi = ((uint64_t)sm_key(sm_first(r, (float)(at.at - 1))) << 32) - 1;
+        before = at.before;
+#pragma unroll 1
+        while (true) {
+          sm_gather<T>(sh, r, x, V, lo, hi);
+          if (sh.n <= kList) break;
+          sm_narrow<T>(sh, r, x, V, counts, target, lo, hi, before);
+        }
+      }
+      SampleSums l;
+      sm_order(sh, r, (int)sh.n, counts && !listed, l);
+      if (listed && step == 0) at.at = (int)target - 1;  // (its sums are masses)
+      else at = sm_find(sh, l, before, target);
+      if (listed) s = l;
     }
-    hit = sm_find_list(sh, l, rule, target);
-    z = (double)hit.mass;
+    const uint64_t e = sh.list[at.at];
+    z = at.upto;
+    if (step == 0) {
+      if (listed) {
+        z = sm_last(sh, s, at.at);
+      } else {  // the row ends there
+        r.low = sm_val((uint32_t)(e >> 32));
+        r.low_last = (int)~(uint32_t)e;
+      }
+      counts = false;
+    }
+    token = (int)~(uint32_t)e;
   }
-  if (threadIdx.x == 0) a.out[row] = hit.index;
+  if (threadIdx.x == 0) a.out[row] = token;
 }
 
 }  // namespace ak
@@ -500,7 +495,7 @@ extern "C" int ak_sample(int dtype, const void* logits, const float* u, int64_t*
                          const float* min_p_rows, float min_p, hipStream_t stream) {
   if (dtype != AK_F32 && dtype != AK_F16 && dtype != AK_BF16) return AK_EINVAL;
   if (rows < 0 || vocab <= 0 || row_stride < 0 || rows > INT_MAX || (rows > 1 && row_stride < vocab)) return AK_EINVAL;
-  if (!temperature_rows && !(temperature >= 0.f && temperature < INFINITY)) return AK_EINVAL;
+  if (!temperature_rows && !(temperature >= 0.f && temperature <= kMaxTemperature)) return AK_EINVAL;
   if (!top_p_rows && top_p != top_p) return AK_EINVAL;
   if (!min_p_rows && min_p != min_p) return AK_EINVAL;
   if (vocab > (1 << 20)) return AK_EUNSUPPORTED;

@@ -13,7 +13,8 @@ greedy: the maximum, lowest index. Every setting is a number or a tensor with on
 The random numbers are the caller's, so a seed gives the same tokens whatever the batch; weights and sums
 are exact to better than 2^-40 and add up in no particular order, so a row and its number always give the
 same token. A row that holds a NaN or nothing but -inf gives -1, as does one whose setting (from a tensor)
-is a NaN or, for the temperature, negative or infinite; a number like that is refused. u below 0 counts as
+is a NaN or, for the temperature, outside 0 .. 1e30; a number like that is refused. +inf counts as the
+largest finite float32. u below 0 counts as
 0, above 1 - 2^-24 as that. Vocabularies up to 2^20. Runs ak_sample (sample.hip).
 """
 from __future__ import annotations
@@ -52,8 +53,8 @@ def kernel_fn(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, t
     k = _setting("top_k", top_k, torch.int32, rows, logits.device)
     p = _setting("top_p", top_p, torch.float32, rows, logits.device)
     m = _setting("min_p", min_p, torch.float32, rows, logits.device)
-    if not torch.is_tensor(t) and not 0.0 <= t <= 3e38:
-        raise ValueError(f"sample: temperature {t} must be finite and not negative")
+    if not torch.is_tensor(t) and not 0.0 <= t <= 1e30:
+        raise ValueError(f"sample: temperature {t} must be from 0 to 1e30")
     for name, v in (("top_p", p), ("min_p", m)):
         if not torch.is_tensor(v) and not 0.0 <= v <= 1.0:
             raise ValueError(f"sample: {name} {v} must be from 0 to 1")
