@@ -14,6 +14,7 @@
 //
 // One block of 16 waves per row:
 //   1. the maximum
+//      With top-k up to kQuickK, or min-p, a bound on what they keep usually leads straight to the list of 3.
 //   2. a histogram of the row over kBins equal steps of log w, from the maximum down to 2^-44 (below, a weight
 //      adds nothing): of masses, or of counts while top-k is to be found
 //   3. the bins' running sums name the bin where a border lies. Where the bins down to it hold few enough
@@ -32,9 +33,10 @@ namespace ak {
 
 constexpr int kSmThreads = 1024;
 constexpr int kSmWaves = kSmThreads / kWave;
-constexpr int kPer = 4;                         // bins or list entries of a thread
-constexpr int kBins = kPer * kSmThreads, kList = kBins;
+constexpr int kBinsPer = 8, kListPer = 4;       // of a thread
+constexpr int kBins = kBinsPer * kSmThreads, kList = kListPer * kSmThreads;
 constexpr int kRanked = 512;                    // lists up to this are ordered by counting, not by a sort network
+constexpr int kQuickK = 512;                    // top-k up to this starts from the threads' maxima
 constexpr float kMaxTemperature = 1e30f;        // differences of floats up to the largest stay tellable
 constexpr float kSpan = 44.0f;                  // octaves of weight that the bins cover
 
@@ -51,7 +53,10 @@ struct SampleArgs {
 
 struct SampleShared {
   uint64_t hist[kBins];
-  uint64_t list[kList];  // (the finer bins' histogram while a bin is cut up)
+  union {
+    uint64_t list[kList];
+    uint64_t fine[kBins];  // finer bins, while a bin is cut up
+  };
   uint64_t red[kSmWaves], red2[kSmWaves];
   uint64_t found[3];     // a border: its entry, the sum up to it, the sum before it
   uint32_t n;
@@ -172,14 +177,16 @@ __device__ __forceinline__ uint64_t sm_block_max(uint64_t v, uint64_t* red) {
   return sm_wave_max(red[lane_id() % kSmWaves]);
 }
 
-// Running sums over kBins values, this thread's four: the sum before them, and up to each.
+// Running sums over the threads' values: the sum before this thread's, and up to each of them.
+template <int PER>
 struct SampleSums {
-  uint64_t before, upto[kPer];
+  uint64_t before, upto[PER];
 };
-__device__ __forceinline__ void sm_sums(SampleShared& sh, const uint64_t (&v)[kPer], SampleSums& s) {
+template <int PER>
+__device__ __forceinline__ void sm_sums(SampleShared& sh, const uint64_t (&v)[PER], SampleSums<PER>& s) {
   uint64_t sum = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) s.upto[i] = sum += v[i];
+  for (int i = 0; i < PER; ++i) s.upto[i] = sum += v[i];
   uint64_t run = sum;
 #pragma unroll 1
   for (int o = 1; o < kWave; o <<= 1) {
@@ -193,52 +200,69 @@ __device__ __forceinline__ void sm_sums(SampleShared& sh, const uint64_t (&v)[kP
 #pragma unroll 1
   for (int i = 0; i < wave_id(); ++i) s.before += sh.red[i];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) s.upto[i] += s.before;
+  for (int i = 0; i < PER; ++i) s.upto[i] += s.before;
+}
+__device__ __forceinline__ void sm_sum_bins(SampleShared& sh, const uint64_t* bins, SampleSums<kBinsPer>& s) {
+  uint64_t v[kBinsPer];
+#pragma unroll
+  for (int i = 0; i < kBinsPer; ++i) v[i] = bins[threadIdx.x * kBinsPer + i];
+  sm_sums(sh, v, s);
+}
+__device__ __forceinline__ void sm_clear(uint64_t* bins) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kSmThreads) bins[i] = 0;
+  __syncthreads();
 }
 // The first of the values whose running sum, with `base` before them all, reaches the target.
 struct SampleBorder {
   int at;
   uint64_t upto, before;
 };
-__device__ __forceinline__ SampleBorder sm_find(SampleShared& sh, const SampleSums& s, uint64_t base, uint64_t target) {
+template <int PER>
+__device__ __forceinline__ SampleBorder sm_find(SampleShared& sh, const SampleSums<PER>& s, uint64_t base,
+                                                uint64_t target) {
   __syncthreads();
-  if (base + s.before < target && base + s.upto[kPer - 1] >= target) {
+  if (base + s.before < target && base + s.upto[PER - 1] >= target) {
     int i = 0;
     uint64_t upto = s.upto[0], before = s.before;
 #pragma unroll
-    for (int j = 1; j < kPer; ++j)
+    for (int j = 1; j < PER; ++j)
       if (base + upto < target) i = j, before = upto, upto = s.upto[j];
-    sh.found[0] = threadIdx.x * kPer + i;
+    sh.found[0] = threadIdx.x * PER + i;
     sh.found[1] = base + upto;
     sh.found[2] = base + before;
   }
   __syncthreads();
   return SampleBorder{(int)sh.found[0], sh.found[1], sh.found[2]};
 }
-
 // The running sum up to value `at`.
-__device__ __forceinline__ uint64_t sm_last(SampleShared& sh, const SampleSums& s, int at) {
+template <int PER>
+__device__ __forceinline__ uint64_t sm_last(SampleShared& sh, const SampleSums<PER>& s, int at) {
   __syncthreads();
-  if ((int)threadIdx.x == at / kPer) sh.found[1] = at % kPer < 2 ? s.upto[at & 1] : s.upto[2 + (at & 1)];
+  if ((int)threadIdx.x == at / PER) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (at % PER == i) sh.found[1] = s.upto[i];
+  }
   __syncthreads();
   return sh.found[1];
 }
 // About how many elements the bins up to `at` hold: counted, or their masses over the weight in a bin's middle.
-__device__ __forceinline__ uint32_t sm_upto(SampleShared& sh, const SampleSums& s, int at, bool counts) {
+__device__ __forceinline__ uint32_t sm_upto(SampleShared& sh, const SampleSums<kBinsPer>& s, int at, bool counts) {
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
   float n = 0.f;
   uint64_t before = s.before;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int b = threadIdx.x * kPer + i;
+  for (int i = 0; i < kBinsPer; ++i) {
+    const int b = threadIdx.x * kBinsPer + i;
     const float in = (float)(s.upto[i] - before);
     if (b <= at) n += counts ? in : in * __builtin_amdgcn_exp2f(((float)b + 0.5f) * (kSpan / kBins) - 42.0f);
     before = s.upto[i];
   }
   n = wave_sum(n);
-  if (lane_id() == 0) atomicAdd(&sh.n, (uint32_t)(n + 0.5f));
+  if (lane_id() == 0 && n >= 0.5f) atomicAdd(&sh.n, (uint32_t)fminf(n + 0.5f, 1e8f));
   __syncthreads();
   return sh.n;
 }
@@ -246,10 +270,8 @@ __device__ __forceinline__ uint32_t sm_upto(SampleShared& sh, const SampleSums& 
 // What an element adds: 1, or its weight.
 template <typename T>
 __device__ __forceinline__ void sm_histogram(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V,
-                                             bool counts, SampleSums& s) {
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kSmThreads) sh.hist[i] = 0;
-  __syncthreads();
+                                             bool counts, SampleSums<kBinsPer>& s) {
+  sm_clear(sh.hist);
   auto add = [&](float v, uint64_t w) {
     atomicAdd((unsigned long long*)&sh.hist[(int)sm_bin(r, v)], (unsigned long long)w);
   };
@@ -263,10 +285,7 @@ __device__ __forceinline__ void sm_histogram(SampleShared& sh, const SampleRow& 
     });
   }
   __syncthreads();
-  uint64_t v[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) v[i] = sh.hist[threadIdx.x * kPer + i];
-  sm_sums(sh, v, s);
+  sm_sum_bins(sh, sh.hist, s);
 }
 
 // Pairs in [lo, hi] of the row, into the list. sh.n: how many there are, which may be more than it holds.
@@ -290,7 +309,8 @@ __device__ __forceinline__ void sm_gather(SampleShared& sh, const SampleRow& r, 
 }
 
 // The list in falling order, and its running sums (of ones, or of weights).
-__device__ __forceinline__ void sm_order(SampleShared& sh, const SampleRow& r, int n, bool counts, SampleSums& s) {
+__device__ __forceinline__ void sm_order(SampleShared& sh, const SampleRow& r, int n, bool counts,
+                                         SampleSums<kListPer>& s) {
   if (n <= kRanked) {
     // an entry's place is the number of larger ones
     const int tid = threadIdx.x;
@@ -322,10 +342,10 @@ __device__ __forceinline__ void sm_order(SampleShared& sh, const SampleRow& r, i
       }
   }
   __syncthreads();
-  uint64_t v[kPer];
+  uint64_t v[kListPer];
 #pragma unroll 1
-  for (int i = 0; i < kPer; ++i) {
-    const int e = threadIdx.x * kPer + i;
+  for (int i = 0; i < kListPer; ++i) {
+    const int e = threadIdx.x * kListPer + i;
     const uint64_t w = e >= n ? 0 : counts ? 1 : sm_fixed(r, sm_val((uint32_t)(sh.list[e] >> 32)));
     v[0] = i == 0 ? w : v[0], v[1] = i == 1 ? w : v[1], v[2] = i == 2 ? w : v[2], v[3] = i == 3 ? w : v[3];
   }
@@ -351,21 +371,16 @@ __device__ __forceinline__ void sm_narrow(SampleShared& sh, const SampleRow& r, 
   lo = ~sm_block_max(z, sh.red2);
   int shift = 0;
   while (((hi - lo) >> shift) >= kBins) ++shift;
-  __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kSmThreads) sh.list[i] = 0;
-  __syncthreads();
+  sm_clear(sh.fine);
   sm_each<T, true>(x, V, [&](float v, int i) {
     if (!(v >= vlo && v <= vhi)) return;
     const uint64_t e = sm_pair(v, i);
     if (e < lo || e > hi) return;
-    atomicAdd((unsigned long long*)&sh.list[(hi - e) >> shift], (unsigned long long)(counts ? 1 : sm_fixed(r, v)));
+    atomicAdd((unsigned long long*)&sh.fine[(hi - e) >> shift], (unsigned long long)(counts ? 1 : sm_fixed(r, v)));
   });
   __syncthreads();
-  uint64_t v[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) v[i] = sh.list[threadIdx.x * kPer + i];
-  SampleSums s;
-  sm_sums(sh, v, s);
+  SampleSums<kBinsPer> s;
+  sm_sum_bins(sh, sh.fine, s);
   const SampleBorder in = sm_find(sh, s, before, target);
   const uint64_t width = (1ull << shift) - 1;
   hi -= (uint64_t)in.at << shift;
@@ -388,21 +403,20 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
   u = u >= 0.f ? fminf(u, 1.0f - 0x1p-24f) : 0.f;
 
   // 1. maximum (v_maximum hands a NaN on, fminf above would lose it: the raw values)
-  float top;
+  float top, mine = -INFINITY;  // of the row, of this thread's elements
   {
-    float m = -INFINITY;
     const int head = min(V, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(S));
     const int nv = (V - head) / T::kVec, tail = head + nv * T::kVec;
-    for (int i = threadIdx.x; i < head; i += kSmThreads) m = __builtin_elementwise_maximum(m, T::to_f(x[i]));
-    for (int i = tail + threadIdx.x; i < V; i += kSmThreads) m = __builtin_elementwise_maximum(m, T::to_f(x[i]));
+    for (int i = threadIdx.x; i < head; i += kSmThreads) mine = __builtin_elementwise_maximum(mine, T::to_f(x[i]));
+    for (int i = tail + threadIdx.x; i < V; i += kSmThreads) mine = __builtin_elementwise_maximum(mine, T::to_f(x[i]));
 #pragma unroll 4
     for (int i = threadIdx.x; i < nv; i += kSmThreads) {
       const u32x4 v = ld16(x + head + (int64_t)i * T::kVec);
 #pragma unroll
-      for (int e = 0; e < T::kVec; ++e) m = __builtin_elementwise_maximum(m, T::lane_elem(v, e));
+      for (int e = 0; e < T::kVec; ++e) mine = __builtin_elementwise_maximum(mine, T::lane_elem(v, e));
     }
-    const uint64_t nan = __builtin_amdgcn_ballot_w64(m != m) ? 1 : 0;
-    const uint64_t best = (uint64_t)sm_key(m) << 1 | nan;
+    const uint64_t nan = __builtin_amdgcn_ballot_w64(mine != mine) ? 1 : 0;
+    const uint64_t best = (uint64_t)sm_key(mine) << 1 | nan;
     const uint64_t all = sm_block_max((nan << 40) | best, sh.red);
     top = all >> 40 ? __builtin_nanf("") : sm_val((uint32_t)(all >> 1));
   }
@@ -431,12 +445,38 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
   // 2, 3. the borders, one after another: top-k (while it is looked for, elements count 1 each), top-p, the
   // token. A list that starts at the row's maximum holds the later borders too.
   bool counts = top_k > 0 && top_k < V, listed = false;
-  SampleSums s;  // of the bins, or of the list
+  SampleSums<kBinsPer> s;
+  SampleSums<kListPer> l;
   uint64_t z = 0;
   int token = -1;
+  const uint64_t least = sm_pair(r.low, r.low_last), most = sm_pair(r.topf, 0);
+  // Short cuts to the list, without a histogram of the row: the top_k-th largest of the threads' maxima is a
+  // bound that at least top_k elements pass, and few more; min-p mostly leaves few elements.
+  const bool quick = counts && top_k <= kQuickK;
+  if (quick || r.min_p > 0.f) {
+    uint64_t lo = least;
+    if (quick) {
+      sm_clear(sh.hist);
+      mine = fminf(mine, FLT_MAX);
+      if (mine >= r.low) atomicAdd((unsigned long long*)&sh.hist[(int)sm_bin(r, mine)], 1ull);
+      __syncthreads();
+      sm_sum_bins(sh, sh.hist, s);
+      if (sm_last(sh, s, kBins - 1) >= (uint64_t)top_k) {
+        const uint64_t bound = sm_pair(sm_first(r, (float)sm_find(sh, s, 0, top_k).at), INT_MAX);
+        if (bound > lo) lo = bound;
+      }
+    }
+    sm_gather<T>(sh, r, x, V, lo, most);
+    listed = sh.n <= (quick ? kList : kRanked);
+    if (listed) {
+      sm_order(sh, r, (int)sh.n, false, l);
+      z = sm_last(sh, l, (counts ? min((uint32_t)top_k, sh.n) : sh.n) - 1);
+      counts = false;
+    }
+  }
 #pragma unroll 1
   for (int step = counts ? 0 : 1; step < 3; ++step) {
-    if (!listed && (step < 2 || z == 0)) {
+    if (!listed && step < 2) {
       sm_histogram<T>(sh, r, x, V, counts, s);
       z = sm_last(sh, s, kBins - 1);  // everything that is left
     }
@@ -444,18 +484,19 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
     const uint64_t target = step == 0   ? min((uint64_t)top_k, z)  // a row with fewer elements ends at its last one
                             : step == 1 ? max((uint64_t)__builtin_ceil((double)top_p * (double)z), (uint64_t)1)
                                         : (uint64_t)((double)u * (double)z) + 1;
-    SampleBorder at = sm_find(sh, s, 0, target);
+    uint64_t before = 0;
     if (!listed) {
-      uint64_t lo = sm_pair(sm_first(r, (float)at.at), INT_MAX), hi = sm_pair(r.topf, 0), before = 0;
-      const uint64_t least = sm_pair(r.low, r.low_last);
-      if (lo < least) lo = least;
-      if (sm_upto(sh, s, at.at, counts) <= kList) {
+      const SampleBorder bin = sm_find(sh, s, 0, target);
+      uint64_t lo = sm_pair(sm_first(r, (float)bin.at), INT_MAX), hi = most;
+      const uint64_t end = sm_pair(r.low, r.low_last);
+      if (lo < end) lo = end;
+      if (step > 0 && sm_upto(sh, s, bin.at, counts) <= kRanked) {
         sm_gather<T>(sh, r, x, V, lo, hi);
         listed = sh.n <= kList;
       }
       if (!listed) {
-        if (at.at > 0) hi = ((uint64_t)sm_key(sm_first(r, (float)(at.at - 1))) << 32) - 1;
-        before = at.before;
+        if (bin.at > 0) hi = ((uint64_t)sm_key(sm_first(r, (float)(bin.at - 1))) << 32) - 1;
+        before = bin.before;
 #pragma unroll 1
         while (true) {
           sm_gather<T>(sh, r, x, V, lo, hi);
@@ -463,21 +504,14 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
           sm_narrow<T>(sh, r, x, V, counts, target, lo, hi, before);
         }
       }
-      SampleSums l;
-      sm_order(sh, r, (int)sh.n, counts && !listed, l);
-      if (listed && step == 0) at.at = (int)target - 1;  // (its sums are masses)
-      else at = sm_find(sh, l, before, target);
-      if (listed) s = l;
+      sm_order(sh, r, (int)sh.n, counts, l);
     }
+    const SampleBorder at = sm_find(sh, l, before, target);
     const uint64_t e = sh.list[at.at];
     z = at.upto;
-    if (step == 0) {
-      if (listed) {
-        z = sm_last(sh, s, at.at);
-      } else {  // the row ends there
-        r.low = sm_val((uint32_t)(e >> 32));
-        r.low_last = (int)~(uint32_t)e;
-      }
+    if (step == 0) {  // the row ends there
+      r.low = sm_val((uint32_t)(e >> 32));
+      r.low_last = (int)~(uint32_t)e;
       counts = false;
     }
     token = (int)~(uint32_t)e;
