@@ -8,7 +8,7 @@
 // and the row is never sorted as a whole.
 //
 // The token is a whole number that a rounding error could change, so weights and sums are exact where it
-// counts: w is computed in 64-bit floating point (2^x by a polynomial, error below 1e-12) and added as
+// counts: w is computed in 64-bit floating point (2^x by a polynomial, error below 1e-13) and added as
 // an integer multiple of 2^-42. Integer sums do not depend on their order, so LDS atomics add them and the
 // token is the same on every run. A row of 2^20 weights stays below 2^62.
 //
@@ -21,7 +21,7 @@
 //      elements, these are gathered as (key, index) pairs and sorted in LDS, and the borders fall out of one
 //      scan. Otherwise the border's own bin is gathered, cut into finer ranges first while it holds too many.
 //      (A top-k border found that way becomes a bound on the row, and step 2 is done again with masses.)
-// What bounds it: the 64-bit weights of a whole row where no top-k spares them, about 28 instructions an
+// What bounds it: the 64-bit weights of a whole row where no top-k spares them, about 25 instructions an
 // element. So everything else an element meets is one or two comparisons: a bin, or min-p, is a range of
 // floats, whose end is found once per row by trying 64 candidates at a time.
 #include <float.h>
@@ -35,9 +35,10 @@ constexpr int kSmThreads = 1024;
 constexpr int kSmWaves = kSmThreads / kWave;
 constexpr int kBinsPer = 8, kListPer = 4;       // of a thread
 constexpr int kBins = kBinsPer * kSmThreads, kList = kListPer * kSmThreads;
+constexpr int kFine = kList;
 constexpr int kRanked = 512;                    // lists up to this are ordered by counting, not by a sort network
 constexpr int kQuickK = 512;                    // top-k up to this starts from the threads' maxima
-constexpr float kMaxTemperature = 1e30f;        // differences of floats up to the largest stay tellable
+constexpr float kMinTemperature = 1e-20f, kMaxTemperature = 1e30f;  // (bins per unit of x stay a float)
 constexpr float kSpan = 44.0f;                  // octaves of weight that the bins cover
 
 struct SampleArgs {
@@ -53,10 +54,8 @@ struct SampleArgs {
 
 struct SampleShared {
   uint64_t hist[kBins];
-  union {
-    uint64_t list[kList];
-    uint64_t fine[kBins];  // finer bins, while a bin is cut up
-  };
+  uint64_t list[kList];
+  uint64_t fine[kFine];  // finer bins, while a bin is cut up
   uint64_t red[kSmWaves], red2[kSmWaves];
   uint64_t found[3];     // a border: its entry, the sum up to it, the sum before it
   uint32_t n;
@@ -81,29 +80,39 @@ struct SampleRow {
   float min_p;
 };
 
-// 2^y for y <= 0: rounded to an integer n plus |f| <= 1/2, the Taylor polynomial of 2^f (its first term
-// left out is below 2.3e-13) and a shift of the exponent.
-__device__ __forceinline__ double sm_exp2(double y) {
-  const double n = __builtin_rint(y), f = y - n;
-  double r = 7.0549116208011232e-09;
-  r = __builtin_fma(r, f, 1.0178086009239699e-07);
-  r = __builtin_fma(r, f, 1.3215486790144309e-06);
-  r = __builtin_fma(r, f, 1.5252733804059841e-05);
-  r = __builtin_fma(r, f, 1.5403530393381608e-04);
-  r = __builtin_fma(r, f, 1.3333558146428443e-03);
-  r = __builtin_fma(r, f, 9.6181291076284772e-03);
-  r = __builtin_fma(r, f, 5.5504108664821576e-02);
-  r = __builtin_fma(r, f, 2.4022650695910069e-01);
-  r = __builtin_fma(r, f, 6.9314718055994529e-01);
-  r = __builtin_fma(r, f, 1.0);
-  return __builtin_ldexp(r, (int)n);
+// (2^f - 1) / f for |f| <= 1/2: interpolated at the nine Chebyshev nodes in long double. 1 + f q(f) is 2^f to
+// 3.7e-14, and 1 at 0.
+// (The instruction itself, its constant in scalar registers: the compiler takes the two-operand form and copies a
+// constant into place before each of them.)
+__device__ __forceinline__ double sm_fma(double a, double b, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+  return d;
 }
+__device__ __forceinline__ double sm_q(double f) {
+  double q = sm_fma(f, 1.0203121156603192e-07, 1.325522487537687e-06);
+  q = sm_fma(q, f, 1.5252686845879443e-05);
+  q = sm_fma(q, f, 0.0001540345585246757);
+  q = sm_fma(q, f, 0.001333355817904356);
+  q = sm_fma(q, f, 0.009618129159402543);
+  q = sm_fma(q, f, 0.055504108664760424);
+  q = sm_fma(q, f, 0.2402265069581299);
+  return sm_fma(q, f, 0.6931471805599453);
+}
+// w of x <= topf
 __device__ __forceinline__ double sm_weight(const SampleRow& r, float x) {
-  return sm_exp2(((double)x - r.top) * r.c);
+  const double y = fmax(((double)x - r.top) * r.c, -999.0), n = __builtin_rint(y), f = y - n;
+  return __builtin_ldexp(__builtin_fma(sm_q(f), f, 1.0), (int)n);
 }
-// Weight in units of 2^-42, rounded to nearest: 2^10 has this unit as its last place. (x within the bins.)
+// w in units of 2^-42, rounded to nearest, for x within the bins: log2 of it is between -2.1 and 42. Adding 1.5 2^52
+// leaves the nearest integer in the low word (and, taken off again, as a double), adding 2^52 the rounded result
+// in the mantissa.
 __device__ __forceinline__ uint64_t sm_fixed(const SampleRow& r, float x) {
-  return __builtin_bit_cast(uint64_t, sm_exp2(((double)x - r.top) * r.c) + 1024.0) - 0x4090000000000000ull;
+  const double y = __builtin_fma((double)x - r.top, r.c, 42.0), t = y + 6755399441055744.0;
+  const double f = y - (t - 6755399441055744.0);
+  uint64_t b = __builtin_bit_cast(uint64_t, __builtin_fma(sm_q(f), f, 1.0));
+  b += (uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, t) << 52;
+  return __builtin_bit_cast(uint64_t, __builtin_bit_cast(double, b) + 4503599627370496.0) & 0xfffffffffffffull;
 }
 // Bin of x <= topf: rises as x falls (each operation rounds monotonically). kBins and more: too light.
 __device__ __forceinline__ float sm_bin(const SampleRow& r, float x) { return (r.topf - x) * r.step; }
@@ -125,6 +134,9 @@ __device__ __forceinline__ float sm_first(const SampleRow& r, float last) {
   return sm_val(hi);
 }
 
+// (v_minimum: fminf takes a second instruction for signalling NaNs)
+__device__ __forceinline__ float sm_finite(float x) { return __builtin_elementwise_minimum(x, FLT_MAX); }
+
 // f(value, index) for every element of the row, 16-byte vectors between an unaligned head and tail, the next two
 // vectors in flight. +infinity counts as the largest finite float. HEAVY: a long f stands in the code once per
 // 32-bit word of a vector, not once per element of it.
@@ -138,7 +150,7 @@ __device__ __forceinline__ void sm_each(const typename T::S* x, int V, F f) {
   auto load = [&](int i) { return ld16(p + (int64_t)min(i, nv - 1) * W); };
   // head and tail: at most W - 1 elements each, on the first lanes of two waves
   const int edge = tid < kWave ? (tid < head ? tid : -1) : (tid - kWave < V - tail ? tail + tid - kWave : -1);
-  if (tid < 2 * kWave && edge >= 0) f(fminf(T::to_f(x[edge]), FLT_MAX), edge);
+  if (tid < 2 * kWave && edge >= 0) f(sm_finite(T::to_f(x[edge])), edge);
   if (nv == 0) return;
   u32x4 next = load(tid), after = load(tid + kSmThreads);
 #pragma unroll 1
@@ -151,12 +163,12 @@ __device__ __forceinline__ void sm_each(const typename T::S* x, int V, F f) {
 #pragma unroll 1
       for (int q = 0; q < 4; ++q) {
 #pragma unroll
-        for (int e = 0; e < W / 4; ++e) f(fminf(T::lane_elem(w, e), FLT_MAX), head + i * W + q * (W / 4) + e);
+        for (int e = 0; e < W / 4; ++e) f(sm_finite(T::lane_elem(w, e)), head + i * W + q * (W / 4) + e);
         w = u32x4{w[1], w[2], w[3], w[0]};
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < W; ++e) f(fminf(T::lane_elem(v, e), FLT_MAX), head + i * W + e);
+      for (int e = 0; e < W; ++e) f(sm_finite(T::lane_elem(v, e)), head + i * W + e);
     }
   }
 }
@@ -202,15 +214,18 @@ __device__ __forceinline__ void sm_sums(SampleShared& sh, const uint64_t (&v)[PE
 #pragma unroll
   for (int i = 0; i < PER; ++i) s.upto[i] += s.before;
 }
-__device__ __forceinline__ void sm_sum_bins(SampleShared& sh, const uint64_t* bins, SampleSums<kBinsPer>& s) {
-  uint64_t v[kBinsPer];
+template <int PER>
+__device__ __forceinline__ void sm_sum_bins(SampleShared& sh, const uint64_t* bins, SampleSums<PER>& s) {
+  uint64_t v[PER];
 #pragma unroll
-  for (int i = 0; i < kBinsPer; ++i) v[i] = bins[threadIdx.x * kBinsPer + i];
+  for (int i = 0; i < PER; ++i) v[i] = bins[threadIdx.x * PER + i];
   sm_sums(sh, v, s);
 }
+template <int PER>
 __device__ __forceinline__ void sm_clear(uint64_t* bins) {
   __syncthreads();
-  for (int i = threadIdx.x; i < kBins; i += kSmThreads) bins[i] = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) bins[threadIdx.x + i * kSmThreads] = 0;
   __syncthreads();
 }
 // The first of the values whose running sum, with `base` before them all, reaches the target.
@@ -271,13 +286,17 @@ __device__ __forceinline__ uint32_t sm_upto(SampleShared& sh, const SampleSums<k
 template <typename T>
 __device__ __forceinline__ void sm_histogram(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V,
                                              bool counts, SampleSums<kBinsPer>& s) {
-  sm_clear(sh.hist);
+  sm_clear<kBinsPer>(sh.hist);
   auto add = [&](float v, uint64_t w) {
     atomicAdd((unsigned long long*)&sh.hist[(int)sm_bin(r, v)], (unsigned long long)w);
   };
   if (counts) {
     sm_each<T, true>(x, V, [&](float v, int) {
       if (v >= r.low) add(v, 1);
+    });
+  } else if (r.low_last == INT_MAX) {
+    sm_each<T, false>(x, V, [&](float v, int) {
+      if (v >= r.low) add(v, sm_fixed(r, v));
     });
   } else {
     sm_each<T, true>(x, V, [&](float v, int i) {
@@ -352,40 +371,71 @@ __device__ __forceinline__ void sm_order(SampleShared& sh, const SampleRow& r, i
   sm_sums(sh, v, s);
 }
 
-// Cuts the pairs [lo, hi], `before` being the sum of the larger ones, to a range around the border that fits the
-// list: a histogram over kBins equal ranges of pairs, as often as it takes. Returns the elements in it, about.
-template <typename T>
-__device__ __forceinline__ void sm_narrow(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V, bool counts,
-                                          uint64_t target, uint64_t& lo, uint64_t& hi, uint64_t& before) {
-  // the range that the elements really take
+// The finer bins of a border's surroundings: equal ranges of the pairs that its elements take. each(f) calls f on
+// this thread's pairs; `before` is the sum of the pairs above them. lo, hi and before become the border's range.
+template <typename E>
+__device__ __forceinline__ void sm_cut(SampleShared& sh, const SampleRow& r, bool counts, uint64_t target, uint64_t& lo,
+                                       uint64_t& hi, uint64_t& before, E each) {
   uint64_t a = 0, z = 0;  // largest, and largest complement
-  const float vlo = sm_val((uint32_t)(lo >> 32)), vhi = sm_val((uint32_t)(hi >> 32));
-  sm_each<T, true>(x, V, [&](float v, int i) {
-    if (!(v >= vlo && v <= vhi)) return;
-    const uint64_t e = sm_pair(v, i);
-    if (e < lo || e > hi) return;
+  each([&](uint64_t e) {
     a = e > a ? e : a;
     z = ~e > z ? ~e : z;
   });
   hi = sm_block_max(a, sh.red);
   lo = ~sm_block_max(z, sh.red2);
   int shift = 0;
-  while (((hi - lo) >> shift) >= kBins) ++shift;
-  sm_clear(sh.fine);
-  sm_each<T, true>(x, V, [&](float v, int i) {
-    if (!(v >= vlo && v <= vhi)) return;
-    const uint64_t e = sm_pair(v, i);
-    if (e < lo || e > hi) return;
-    atomicAdd((unsigned long long*)&sh.fine[(hi - e) >> shift], (unsigned long long)(counts ? 1 : sm_fixed(r, v)));
+  while (((hi - lo) >> shift) >= kFine) ++shift;
+  sm_clear<kListPer>(sh.fine);
+  const uint64_t top = hi;
+  each([&](uint64_t e) {
+    atomicAdd((unsigned long long*)&sh.fine[(top - e) >> shift],
+              (unsigned long long)(counts ? 1 : sm_fixed(r, sm_val((uint32_t)(e >> 32)))));
   });
   __syncthreads();
-  SampleSums<kBinsPer> s;
+  SampleSums<kListPer> s;
   sm_sum_bins(sh, sh.fine, s);
   const SampleBorder in = sm_find(sh, s, before, target);
   const uint64_t width = (1ull << shift) - 1;
   hi -= (uint64_t)in.at << shift;
   if (hi >= width && hi - width > lo) lo = hi - width;
   before = in.before;
+}
+// ... of the row's pairs in [lo, hi], too many for the list
+template <typename T>
+__device__ __forceinline__ void sm_narrow(SampleShared& sh, const SampleRow& r, const typename T::S* x, int V, bool counts,
+                                          uint64_t target, uint64_t& lo, uint64_t& hi, uint64_t& before) {
+  const uint64_t lo0 = lo, hi0 = hi;
+  const float vlo = sm_val((uint32_t)(lo >> 32)), vhi = sm_val((uint32_t)(hi >> 32));
+  sm_cut(sh, r, counts, target, lo, hi, before, [&](auto f) {
+    sm_each<T, true>(x, V, [&](float v, int i) {
+      if (!(v >= vlo && v <= vhi)) return;
+      const uint64_t e = sm_pair(v, i);
+      if (e >= lo0 && e <= hi0) f(e);
+    });
+  });
+}
+// ... of the list, too many to be ordered by counting: the pairs outside the border's range leave it
+__device__ __forceinline__ void sm_thin(SampleShared& sh, const SampleRow& r, bool counts, uint64_t target,
+                                        uint64_t& before) {
+  uint64_t mine[kListPer], lo, hi;
+  const int n = (int)sh.n;
+#pragma unroll
+  for (int i = 0; i < kListPer; ++i) {
+    const int at = threadIdx.x + i * kSmThreads;
+    mine[i] = at < n ? sh.list[at] : 0;  // (no pair is 0)
+  }
+  sm_cut(sh, r, counts, target, lo, hi, before, [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < kListPer; ++i)
+      if (mine[i]) f(mine[i]);
+  });
+  __syncthreads();
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kListPer; ++i)
+    if (mine[i] >= lo && mine[i] <= hi && mine[i]) sh.list[atomicAdd(&sh.n, 1u)] = mine[i];
+  __syncthreads();
 }
 
 template <typename T>
@@ -436,8 +486,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
     return;
   }
   r.top = r.topf;
-  r.c = 1.4426950408889634 / (double)t;
-  r.step = (float)fmin(r.c * (kBins / (double)kSpan), 1e30);
+  r.c = 1.4426950408889634 / (double)fmaxf(t, kMinTemperature);
+  r.step = (float)(r.c * (kBins / (double)kSpan));
   r.min_p = fminf(r.min_p, 1.0f);
   r.low = sm_first(r, kBins - 1);
   r.low_last = INT_MAX;
@@ -456,7 +506,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
   if (quick || r.min_p > 0.f) {
     uint64_t lo = least;
     if (quick) {
-      sm_clear(sh.hist);
+      sm_clear<kBinsPer>(sh.hist);
       mine = fminf(mine, FLT_MAX);
       if (mine >= r.low) atomicAdd((unsigned long long*)&sh.hist[(int)sm_bin(r, mine)], 1ull);
       __syncthreads();
@@ -503,6 +553,8 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
           if (sh.n <= kList) break;
           sm_narrow<T>(sh, r, x, V, counts, target, lo, hi, before);
         }
+#pragma unroll 1
+        while (sh.n > kRanked) sm_thin(sh, r, counts, target, before);
       }
       sm_order(sh, r, (int)sh.n, counts, l);
     }

@@ -395,7 +395,7 @@ int ak_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_c
  *   top-k: the first top_k (top_k <= 0: all)
  *   top-p: the shortest prefix whose mass reaches top_p of theirs, one element at least (top_p >= 1: all)
  *   the token: the first element whose running mass exceeds u times the mass kept
- * temperature 0 takes the maximum (lowest index); 1e30 is the highest. u: fp32 [rows], taken as 0 below 0 and
+ * temperature 0 takes the maximum (lowest index); others count as 1e-20 at least, and 1e30 is the highest. u: fp32 [rows], taken as 0 below 0 and
  * as 1 - 2^-24 above it. Each setting is a scalar, or an array with one value per row where its _rows pointer is not NULL.
  * tokens: int64 [rows]; -1 for a row that holds a NaN, one whose maximum is -infinity and one with a setting
  * from an array that is a NaN or, for the temperature, outside 0 .. 1e30 (as scalars: AK_EINVAL).
