@@ -41,6 +41,8 @@ constexpr int kQuickK = 512;                    // top-k up to this starts from 
 constexpr float kMinTemperature = 1e-20f, kMaxTemperature = 1e30f;  // (bins per unit of x stay a float)
 constexpr float kSpan = 44.0f;                  // octaves of weight that the bins cover
 
+static_assert(2 * kRanked == kSmThreads, "two threads an entry");
+
 struct SampleArgs {
   const void* x;
   int64_t stride;
@@ -54,7 +56,7 @@ struct SampleArgs {
 
 struct SampleShared {
   uint64_t hist[kBins];
-  uint64_t list[kList];
+  alignas(16) uint64_t list[kList];
   uint64_t fine[kFine];  // finer bins, while a bin is cut up
   uint64_t red[kSmWaves], red2[kSmWaves];
   uint64_t found[3];     // a border: its entry, the sum up to it, the sum before it
@@ -331,15 +333,23 @@ __device__ __forceinline__ void sm_gather(SampleShared& sh, const SampleRow& r, 
 __device__ __forceinline__ void sm_order(SampleShared& sh, const SampleRow& r, int n, bool counts,
                                          SampleSums<kListPer>& s) {
   if (n <= kRanked) {
-    // an entry's place is the number of larger ones
-    const int tid = threadIdx.x;
-    const uint64_t me = tid < n ? sh.list[tid] : 0;
-    int place = 0;
-    if (tid < (n + kWave - 1) / kWave * kWave)
-#pragma unroll 4
-      for (int i = 0; i < n; ++i) place += sh.list[i] > me;
+    // an entry's place is the number of larger ones: two threads an entry, one half of the list each
+    const int me_at = threadIdx.x % kRanked, part = threadIdx.x / kRanked;
+    const uint64_t me = me_at < n ? sh.list[me_at] : 0;
+    if (threadIdx.x < 4) sh.list[n + threadIdx.x] = 0;  // (kList is larger)
     __syncthreads();
-    if (tid < n) sh.list[place] = me;
+    const int half = (n + 3) / 4 * 2;
+    uint32_t place = 0;
+    if (me_at < (n + kWave - 1) / kWave * kWave)
+#pragma unroll 2
+      for (int i = part * half; i < (part + 1) * half; i += 2) {
+        const u32x4 p = ld16(&sh.list[i]);
+        place += ((uint64_t)p[1] << 32 | p[0]) > me;
+        place += ((uint64_t)p[3] << 32 | p[2]) > me;
+      }
+    if (part) sh.fine[me_at] = place;
+    __syncthreads();
+    if (!part && me_at < n) sh.list[place + (uint32_t)sh.fine[me_at]] = me;
   } else {
     int n2 = kRanked;
     while (n2 < n) n2 <<= 1;
