@@ -27,6 +27,15 @@ from . import _ops, _paged
 KERNEL_TYPE = "kv_append"
 
 
+def _explain_tables(k: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> None:
+    if not (cos.is_cuda and sin.is_cuda):
+        raise RuntimeError("kv_append: no CPU path (tensors must be on the GPU)")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32 or cos.device != k.device or sin.device != k.device:
+        raise ValueError(f"kv_append: cos and sin must be float32 on {k.device}")
+    raise ValueError(f"kv_append: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [positions, rot_dim / 2] "
+                     f"with rot_dim from 2 to {k.shape[2]}")
+
+
 def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
               page_table: torch.Tensor, q_starts: torch.Tensor, kv_lens: torch.Tensor,
               cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, q: torch.Tensor | None = None,
@@ -35,27 +44,22 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
         _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, k=k, v=v)
     else:
         _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, k=k, v=v, q=q)
-    if k.shape[1] != k_cache.shape[1] or v.shape[1] != k_cache.shape[1]:
-        raise ValueError(f"kv_append: k {tuple(k.shape)} and v {tuple(v.shape)} for {k_cache.shape[1]} KV heads")
+    heads = k_cache.shape[1]
+    if k.shape[1] != heads or v.shape[1] != heads:
+        raise ValueError(f"kv_append: k {tuple(k.shape)} and v {tuple(v.shape)} for {heads} KV heads")
     for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
         if 0 in t.stride() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"kv_append: {name} is an expanded view (strides {t.stride()}): its slots share memory")
-    if (cos is None) != (sin is None):
-        raise ValueError("kv_append: cos and sin come together")
-    if cos is None:
-        if q is not None:
-            raise ValueError("kv_append: q without cos and sin has nothing done to it")
-    else:
-        dev = k.get_device()
-        if cos.get_device() < 0 or sin.get_device() < 0:
-            raise RuntimeError("kv_append: no CPU path (tensors must be on the GPU)")
-        if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.get_device() != dev
-                or sin.get_device() != dev):
-            raise ValueError(f"kv_append: cos and sin must be float32 on {k.device}")
-        if cos.dim() != 2 or cos.shape != sin.shape or not 0 < 2 * cos.shape[1] <= k.shape[2]:
-            raise ValueError(f"kv_append: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be "
-                             f"[positions, rot_dim / 2] with rot_dim from 2 to {k.shape[2]}")
+    if cos is not None and sin is not None:
+        dev, shape = k.get_device(), cos.shape
+        if not (cos.get_device() == sin.get_device() == dev and cos.dtype is sin.dtype is torch.float32
+                and shape == sin.shape and len(shape) == 2 and 0 < 2 * shape[1] <= k.shape[2]):
+            _explain_tables(k, cos, sin)
         cos, sin = cos.contiguous(), sin.contiguous()
+    elif cos is not sin:
+        raise ValueError("kv_append: cos and sin come together")
+    elif q is not None:
+        raise ValueError("kv_append: q without cos and sin has nothing done to it")
     k, v = _paged.row_operand(k), _paged.row_operand(v)
     q_out = None
     if q is not None:

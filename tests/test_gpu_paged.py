@@ -443,7 +443,7 @@ def test_workspace_too_small_is_refused(gpu):
     need = _lib.load().ak_paged_attn_workspace_bytes(_lib.AK_BF16, 1, 1, 4, 2, 64, 8, b.width)
     assert need > 0
     o = torch.empty_like(q)
-    st2, st3 = _ops._I64x2(*q.stride()[:2]), _ops._I64x3(*kc.stride()[:3])
+    st2, st3 = _ops._strides(q.stride()), _ops._strides(kc.stride())
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
     for ptr, n in ((ws.data_ptr(), need - 1), (None, need), (ws.data_ptr() + 8, need)):
         with pytest.raises(AkError, match="invalid argument"):
