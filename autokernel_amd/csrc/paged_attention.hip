@@ -1194,15 +1194,9 @@ static PaPlan pa_plan(int dtype, int64_t T, int64_t B, int64_t Hq, int64_t Hk, i
     p.items[1] = (rows / kPtRows + std::min(seqs, rows / (kPaSplitRows + 1))) * Hk;
   }
   if (keys > kPaMinSliced) {
-#ifndef PA_T1
-#define PA_T1 512
-#endif
-#ifndef PA_T0
-#define PA_T0 1536
-#endif
-    p.target[0] = PA_T0;
+    p.target[0] = 1536;
     // two tiles per CU at a time; four times that many are work enough unsliced
-    if (tiles && rows / kPtRows * Hk < 4 * 512) p.target[1] = PA_T1;
+    if (tiles && rows / kPtRows * Hk < 4 * 512) p.target[1] = 512;
   }
   const int64_t row = (D + 3) / 4 * 4 + 2;
   for (int c = 0; c < 2; ++c)
@@ -1267,8 +1261,9 @@ static int launch_fast(const PaArgs& a, const PaPlan& p, void* ws, hipStream_t s
 
 static bool pa_sizes_ok(int64_t T, int64_t B, int64_t Hq, int64_t Hk, int64_t D) {
   if (T < 0 || B < 0 || Hq < 0 || Hk <= 0 || D <= 0 || Hq % Hk != 0 || Hq > 65536) return false;
-  return T <= INT_MAX && B < INT_MAX && T * Hq < (int64_t)1 << 31 && (std::min(B, T) + T * (Hq / Hk)) * Hk < (int64_t)1 << 24;
+  return T <= INT_MAX && B < INT_MAX && T * Hq < (int64_t)1 << 31 && std::min(B, T) * Hk < (int64_t)1 << 31;
 }
+static bool pa_plan_fits(const PaPlan& p) { return grid_fits(p.items[0] + p.items[1], 8 * kWave); }
 
 }  // namespace ak
 
@@ -1281,8 +1276,9 @@ extern "C" int64_t ak_paged_attn_workspace_bytes(int dtype, int64_t T, int64_t B
   if (dtype != AK_F32 && dtype != AK_F16 && dtype != AK_BF16) return 0;
   if (!pa_sizes_ok(T, B, Hq, Hkv, D) || T == 0 || B == 0 || Hq == 0 || page_size <= 0 || max_pages < 0) return 0;
   if (page_size > INT_MAX || max_pages > INT_MAX) return 0;
-  return std::max(pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, D == 64 || D == 128).bytes(),
-                  pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, false).bytes());
+  const PaPlan f = pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, D == 64 || D == 128);
+  const PaPlan g = pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, false);
+  return std::max(pa_plan_fits(f) ? f.bytes() : 0, pa_plan_fits(g) ? g.bytes() : 0);
 }
 
 extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_cache, void* o,
@@ -1327,6 +1323,7 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
   for (const int64_t x : {a.kcp, a.vcp})
     if (x < 0 || x >= (int64_t)1 << 31) fast = false;
   const PaPlan p = pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, fast);
+  if (!pa_plan_fits(p)) return AK_EINVAL;
   AK_DISPATCH(dtype, T_, {
     return fast ? launch_fast<T_>(a, p, workspace, stream) : launch_general<T_>(a, p, workspace, stream);
   });
