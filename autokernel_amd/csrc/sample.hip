@@ -119,16 +119,28 @@ __device__ __forceinline__ uint64_t sm_fixed(const SampleRow& r, float x) {
 // Bin of x <= topf: rises as x falls (each operation rounds monotonically). kBins and more: too light.
 __device__ __forceinline__ float sm_bin(const SampleRow& r, float x) { return (r.topf - x) * r.step; }
 
-// Smallest float of bin `last` or an earlier one with w >= min_p: 64 candidates a round, on every wave. (topf is one.)
+// Smallest float of bin `last` or an earlier one with w >= min_p, on every wave: 64 candidates a round, the first
+// round next to where it should be. (topf is one.)
 __device__ __forceinline__ float sm_first(const SampleRow& r, float last) {
   uint32_t lo = 0, hi = sm_key(r.topf);  // in (lo, hi]; hi is one
+  const auto is = [&](uint32_t key) {
+    const float v = sm_val(key);
+    return sm_bin(r, v) < last + 1.0f && (r.min_p <= 0.f || sm_weight(r, v) >= (double)r.min_p);
+  };
+  float guess = r.topf - (last + 1.0f) / r.step;
+  if (r.min_p > 0.f) guess = fmaxf(guess, r.topf + __builtin_amdgcn_logf(r.min_p) / (float)r.c);
+  const uint32_t near = sm_key(guess);
+  if (near > kWave && near + kWave < hi) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64(is(near - kWave / 2 + lane_id()));
+    const int first = m ? __builtin_ctzll(m) : kWave;
+    if (first > 0) lo = near - kWave / 2 + first - 1;
+    if (first < kWave) hi = near - kWave / 2 + first;
+  }
 #pragma unroll 1
   while (hi - lo > 1) {
     const uint32_t step = max(1u, (hi - lo) / kWave);
-    const float v = sm_val(lo + step * (lane_id() + 1));
     const bool past = step * (uint64_t)(lane_id() + 1) >= hi - lo;
-    const bool is = past || (sm_bin(r, v) < last + 1.0f && (r.min_p <= 0.f || sm_weight(r, v) >= (double)r.min_p));
-    const uint64_t m = __builtin_amdgcn_ballot_w64(is);  // candidates rise: all after the first
+    const uint64_t m = __builtin_amdgcn_ballot_w64(past || is(lo + step * (lane_id() + 1)));  // all after the first
     const int first = m ? __builtin_ctzll(m) : kWave;
     if (first < kWave) hi = min(hi, lo + step * (first + 1));
     lo += step * first;
@@ -191,6 +203,23 @@ __device__ __forceinline__ uint64_t sm_block_max(uint64_t v, uint64_t* red) {
   return sm_wave_max(red[lane_id() % kSmWaves]);
 }
 
+// v plus the lower lanes' values: within rows of 16 lanes by row_shr, then each row's last lane to the rows after
+// it by row_bcast (a shuffle goes through LDS, twice for 64 bits).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t sm_scan_step(uint64_t v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, ROWS, 0xf, false);
+  return v + ((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
+__device__ __forceinline__ uint64_t sm_wave_scan(uint64_t v) {
+  v = sm_scan_step<0x111, 0xf>(v);
+  v = sm_scan_step<0x112, 0xf>(v);
+  v = sm_scan_step<0x114, 0xf>(v);
+  v = sm_scan_step<0x118, 0xf>(v);
+  v = sm_scan_step<0x142, 0xa>(v);
+  return sm_scan_step<0x143, 0xc>(v);
+}
+
 // Running sums over the threads' values: the sum before this thread's, and up to each of them.
 template <int PER>
 struct SampleSums {
@@ -201,18 +230,14 @@ __device__ __forceinline__ void sm_sums(SampleShared& sh, const uint64_t (&v)[PE
   uint64_t sum = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) s.upto[i] = sum += v[i];
-  uint64_t run = sum;
-#pragma unroll 1
-  for (int o = 1; o < kWave; o <<= 1) {
-    const uint64_t w = __shfl_up((unsigned long long)run, o, kWave);
-    if (lane_id() >= o) run += w;
-  }
+  const uint64_t run = sm_wave_scan(sum);
   __syncthreads();
   if (lane_id() == kWave - 1) sh.red[wave_id()] = run;
   __syncthreads();
-  s.before = run - sum;
-#pragma unroll 1
-  for (int i = 0; i < wave_id(); ++i) s.before += sh.red[i];
+  // the waves before this one: their totals, one a lane
+  const uint64_t waves = sm_wave_scan(lane_id() < wave_id() ? sh.red[lane_id() % kSmWaves] : 0);
+  s.before = run - sum + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(waves >> 32), kWave - 1) << 32 |
+                          (uint32_t)__builtin_amdgcn_readlane((int)waves, kWave - 1));
 #pragma unroll
   for (int i = 0; i < PER; ++i) s.upto[i] += s.before;
 }
@@ -230,7 +255,7 @@ __device__ __forceinline__ void sm_clear(uint64_t* bins) {
   for (int i = 0; i < PER; ++i) bins[threadIdx.x + i * kSmThreads] = 0;
   __syncthreads();
 }
-// The first of the values whose running sum, with `base` before them all, reaches the target.
+// The first of the values whose running sum, with `base` before them all, reaches the target; at is -1 if none does.
 struct SampleBorder {
   int at;
   uint64_t upto, before;
@@ -248,6 +273,8 @@ __device__ __forceinline__ SampleBorder sm_find(SampleShared& sh, const SampleSu
     sh.found[0] = threadIdx.x * PER + i;
     sh.found[1] = base + upto;
     sh.found[2] = base + before;
+  } else if (threadIdx.x == kSmThreads - 1 && base + s.upto[PER - 1] < target) {
+    sh.found[0] = ~0ull;
   }
   __syncthreads();
   return SampleBorder{(int)sh.found[0], sh.found[1], sh.found[2]};
@@ -516,13 +543,18 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
   if (quick || r.min_p > 0.f) {
     uint64_t lo = least;
     if (quick) {
-      sm_clear<kBinsPer>(sh.hist);
-      mine = fminf(mine, FLT_MAX);
-      if (mine >= r.low) atomicAdd((unsigned long long*)&sh.hist[(int)sm_bin(r, mine)], 1ull);
+      // coarse bins, one a thread: bin b is kBinsPer of the row's
+      sh.hist[threadIdx.x] = 0;
       __syncthreads();
-      sm_sum_bins(sh, sh.hist, s);
-      if (sm_last(sh, s, kBins - 1) >= (uint64_t)top_k) {
-        const uint64_t bound = sm_pair(sm_first(r, (float)sm_find(sh, s, 0, top_k).at), INT_MAX);
+      mine = fminf(mine, FLT_MAX);
+      if (mine >= r.low) atomicAdd((unsigned long long*)&sh.hist[(int)sm_bin(r, mine) / kBinsPer], 1ull);
+      __syncthreads();
+      const uint64_t v[1] = {sh.hist[threadIdx.x]};
+      SampleSums<1> c;
+      sm_sums(sh, v, c);
+      const int bin = sm_find(sh, c, 0, top_k).at;
+      if (bin >= 0) {
+        const uint64_t bound = sm_pair(sm_first(r, (float)(bin * kBinsPer + kBinsPer - 1)), INT_MAX);
         if (bound > lo) lo = bound;
       }
     }

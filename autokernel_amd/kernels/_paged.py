@@ -11,11 +11,11 @@ _I32 = torch.int32
 
 
 def check(op: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, q_starts: torch.Tensor,
-          kv_lens: torch.Tensor, **rows: torch.Tensor) -> None:
-    """ValueError / RuntimeError unless the cache, the index arrays and the row tensors ([T, heads, D]) fit
-    together on one GPU. One expression for the calls that do (7 us less of CPU than the rules one by one);
-    _explain finds what is wrong with the others."""
-    ref = next(iter(rows.values()))
+          kv_lens: torch.Tensor, names: str, *rows: torch.Tensor) -> None:
+    """ValueError / RuntimeError unless the cache, the index arrays and the row tensors ([T, heads, D], one letter of
+    `names` each) fit together on one GPU. One expression for the calls that do (7 us less of CPU than the rules
+    one by one); _explain finds what is wrong with the others."""
+    ref = rows[0]
     dev, dt, shape, cache, table = ref.get_device(), ref.dtype, ref.shape, k_cache.shape, page_table.shape
     if (dev >= 0 and dt in _DTYPES and len(cache) == 4 and len(shape) == 3 and len(table) == 2
             and cache == v_cache.shape and k_cache.dtype is dt and v_cache.dtype is dt
@@ -26,17 +26,14 @@ def check(op: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: tor
             and v_cache.stride(3) == 1 and kv_lens.shape == table[:1] and q_starts.shape == (table[0] + 1,)
             and q_starts.stride(0) == 1 and (kv_lens.stride(0) == 1 or table[0] <= 1)
             and (page_table.stride(1) == 1 or table[1] <= 1) and (page_table.stride(0) >= table[1] or table[0] <= 1)
-            and table[1] * cache[2] < 1 << 31):
-        for t in rows.values():
-            if t is not ref:
-                s = t.shape
-                if not (len(s) == 3 and s[0] == shape[0] and s[2] == cache[3] and t.dtype is dt
-                        and t.get_device() == dev):
-                    break
+            and table[1] * cache[2] < 1 << 31 and shape[2] == cache[3]):
+        for t in rows[1:]:
+            s = t.shape
+            if not (len(s) == 3 and s[0] == shape[0] and s[2] == cache[3] and t.dtype is dt and t.get_device() == dev):
+                break
         else:
-            if shape[2] == cache[3]:
-                return
-    _explain(op, k_cache, v_cache, page_table, q_starts, kv_lens, **rows)
+            return
+    _explain(op, k_cache, v_cache, page_table, q_starts, kv_lens, **dict(zip(names, rows)))
 
 
 def _explain(op: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, q_starts: torch.Tensor,
@@ -86,4 +83,4 @@ def _explain(op: str, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: 
 
 def row_operand(t: torch.Tensor) -> torch.Tensor:
     """[T, heads, D] with a contiguous last dim (a column slice of a fused projection is read in place)."""
-    return t if t.shape[2] <= 1 or t.stride(2) == 1 else t.contiguous()
+    return t if t.stride(2) == 1 or t.shape[2] <= 1 else t.contiguous()

@@ -41,9 +41,9 @@ def kernel_fn(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: 
               cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, q: torch.Tensor | None = None,
               interleaved: bool = True) -> torch.Tensor | None:
     if q is None:
-        _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, k=k, v=v)
+        _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, "kv", k, v)
     else:
-        _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, k=k, v=v, q=q)
+        _paged.check("kv_append", k_cache, v_cache, page_table, q_starts, kv_lens, "kvq", k, v, q)
     heads = k_cache.shape[1]
     if k.shape[1] != heads or v.shape[1] != heads:
         raise ValueError(f"kv_append: k {tuple(k.shape)} and v {tuple(v.shape)} for {heads} KV heads")

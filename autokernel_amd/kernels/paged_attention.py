@@ -27,7 +27,7 @@ KERNEL_TYPE = "paged_attention"
 def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
               q_starts: torch.Tensor, kv_lens: torch.Tensor, sm_scale: float | None = None,
               out: torch.Tensor | None = None) -> torch.Tensor:
-    _paged.check("paged_attention", k_cache, v_cache, page_table, q_starts, kv_lens, q=q)
+    _paged.check("paged_attention", k_cache, v_cache, page_table, q_starts, kv_lens, "q", q)
     if q.shape[1] % k_cache.shape[1]:
         raise ValueError(f"paged_attention: {q.shape[1]} query heads not a multiple of {k_cache.shape[1]} KV heads")
     scale = float(q.shape[2] ** -0.5 if sm_scale is None else sm_scale)
