@@ -38,7 +38,7 @@ struct PaArgs {
   void* o;
   PaClass c[2];    // few rows, many rows
   int split_rows;  // most rows (new tokens times group) of a sequence of class 0
-  FastDiv f_hq;
+  FastDiv f_units;  // pa_merge's units of a token
   int64_t qst, qsh, ost, osh;            // row and head strides (elements)
   int64_t kcp, kch, kct, vcp, vch, vct;  // cache: page, head, slot strides
   int Hq, Hk, G, D, Dp, vec;  // Dp: floats of a partial row, D rounded up to 4
@@ -282,18 +282,35 @@ __global__ __launch_bounds__(kPaThreads) void pa_general(const PaArgs a) {
                                   it.nsplit == 1 ? INT_MAX : lo + it.chunk);
 }
 
-// Sliced rows: W waves per (row, query head). A group of 16 lanes adds the partials of slices g, g + 4 W, ..
-// (lane c: dims 4 c .. 4 c + 3 of each 64), then the groups' sums combine in group order. Four groups of one
-// wave for many rows; with few rows sixteen, so that 64 slices' partials are in flight at once. The grid is
-// bounded and walks the rows: in most calls with many rows nothing is sliced and it ends at once.
-// JN: 64s of head_dim.
-template <typename T, int BM0, int BM1, int JN, int W>
+// Sliced rows: the partials of each (row, query head), added in slice order by groups of 16 lanes (lane c: dims
+// 4 c .. 4 c + 3 of each 64; JN: 64s of head_dim), four slices in flight. With many rows a group has a row to
+// itself (WIDE false: a wave takes four heads of one token); with few, the block's sixteen groups share a row,
+// so that 64 slices' partials are in flight at once, and combine in group order. The grid is bounded and walks the
+// rows: in most calls with many rows nothing is sliced and it ends at once.
+template <int JN>
+struct PaSum {
+  float m, l, acc[JN][4];  // exp2 base, sum, weighted values
+};
+// acc = acc, then x, to the common base
+template <int JN>
+__device__ __forceinline__ void pa_add(PaSum<JN>& s, float m, float l, const f32x4 (&v)[JN]) {
+  if (m == -INFINITY && l == 0.f) return;  // a slice without a key that the row sees
+  const float m_new = nan_max(s.m, m);
+  const float f0 = s.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s.m - m_new);
+  const float f1 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+  s.m = m_new;
+  s.l = s.l * f0 + l * f1;
+#pragma unroll
+  for (int j = 0; j < JN; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s.acc[j][e] = s.acc[j][e] * f0 + v[j][e] * f1;
+}
+template <typename T, int BM0, int BM1, int JN, bool WIDE>
 __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
   using S = typename T::S;
-  constexpr int NG = 4 * W, NR = kPaWaves / W;  // groups of a row, rows of a block
-  __shared__ float so[kPaWaves * 4][64 * JN + 4], sm[kPaWaves * 4], sl[kPaWaves * 4];
-  const int lane = lane_id(), c = lane & 15;
-  const int slot_in = pa_uniform(wave_id()) / W, g = (wave_id() % W) * 4 + lane / 16;
+  constexpr int NG = WIDE ? 4 * kPaWaves : 1;  // groups of a row
+  __shared__ float so[WIDE ? NG : 1][64 * JN + 4], sm[NG], sl[NG];
+  const int lane = lane_id(), c = lane & 15, grp = threadIdx.x >> 4;
   const PaBatch x{pa_lane_seq(a.s, lane)};
   const int chunk0 = pa_chunk<BM0, 0>(a, x), chunk1 = pa_chunk<BM1, 1>(a, x);
   bool sliced = false;
@@ -312,104 +329,103 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
   };
   int n64[2], upto64[2];
   items(x.q, n64, upto64);
-  const int64_t total = (int64_t)a.s.T * a.Hq;
-  for (int64_t block = blockIdx.x; block * NR < total; block += gridDim.x) {
-    const int64_t row = block * NR + slot_in;
-    const int tok = pa_uniform((int)fdiv((uint32_t)min(row, total - 1), a.f_hq)), h = (int)(row - (int64_t)tok * a.Hq);
-    // the row's sequence, and the items of its class before it
+  // a unit: one (token, head) for the block, or four heads of a token for the wave
+  const int64_t units = (int64_t)a.s.T * (WIDE ? a.Hq : (a.Hq + 3) / 4);
+  const int64_t step = (int64_t)gridDim.x * (WIDE ? 1 : kPaWaves);
+  for (int64_t unit = WIDE ? blockIdx.x : (int64_t)blockIdx.x * kPaWaves + pa_uniform(wave_id()); unit < units;
+       unit += step) {
+    const int tok = pa_uniform((int)fdiv((uint32_t)unit, a.f_units));
+    const int h = WIDE ? (int)unit - tok * a.Hq : 4 * ((int)unit - tok * ((a.Hq + 3) / 4)) + lane / 16;
+    // the token's sequence, and the items of its class before it
     PaSeq q{0, 0, 0, false};
     int cls = 0, nsplit = 1;
     uint32_t first = 0, before[2] = {0, 0};
-    if (row < total)
-      pa_each(a, x, [&](int i, const PaSeq& s) {
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(tok >= s.t0 && tok < s.t0 + s.n);
-        int n[2] = {n64[0], n64[1]}, upto[2] = {upto64[0], upto64[1]};
-        if (i > 0) items(s, n, upto);
-        if (!hit) {
-          before[0] += (uint32_t)__builtin_amdgcn_readlane(upto[0], kWave - 1);
-          before[1] += (uint32_t)__builtin_amdgcn_readlane(upto[1], kWave - 1);
-          return false;
-        }
-        const int l = __builtin_ctzll(hit);
-        q.t0 = __builtin_amdgcn_readlane(s.t0, l);
-        q.n = __builtin_amdgcn_readlane(s.n, l);
-        q.len = __builtin_amdgcn_readlane(s.len, l);
-        q.overlong = __builtin_amdgcn_readlane((int)s.overlong, l) != 0;
-        cls = q.n * a.G <= a.split_rows ? 0 : 1;
-        nsplit = pa_splits(q.len, cls ? chunk1 : chunk0);
-        first = before[cls] + (uint32_t)__builtin_amdgcn_readlane(cls ? upto[1] - n[1] : upto[0] - n[0], l);
-        return true;
-      });
-    const int bm = cls ? BM1 : BM0;
+    pa_each(a, x, [&](int i, const PaSeq& s) {
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(tok >= s.t0 && tok < s.t0 + s.n);
+      int n[2] = {n64[0], n64[1]}, upto[2] = {upto64[0], upto64[1]};
+      if (i > 0) items(s, n, upto);
+      if (!hit) {
+        before[0] += (uint32_t)__builtin_amdgcn_readlane(upto[0], kWave - 1);
+        before[1] += (uint32_t)__builtin_amdgcn_readlane(upto[1], kWave - 1);
+        return false;
+      }
+      const int l = __builtin_ctzll(hit);
+      q.t0 = __builtin_amdgcn_readlane(s.t0, l);
+      q.n = __builtin_amdgcn_readlane(s.n, l);
+      q.len = __builtin_amdgcn_readlane(s.len, l);
+      q.overlong = __builtin_amdgcn_readlane((int)s.overlong, l) != 0;
+      cls = q.n * a.G <= a.split_rows ? 0 : 1;
+      nsplit = pa_splits(q.len, cls ? chunk1 : chunk0);
+      first = before[cls] + (uint32_t)__builtin_amdgcn_readlane(cls ? upto[1] - n[1] : upto[0] - n[0], l);
+      return true;
+    });
+    if (nsplit == 1) continue;  // (the same for the whole block where it shares a unit)
+    const int bm = cls ? BM1 : BM0, tiles = (q.n * a.G + bm - 1) / bm;
     const PaClass& cl = a.c[cls];
-    float m = -INFINITY, l = 0.f, acc[JN][4];
+    const int hk = (int)fdiv((uint32_t)h, a.f_g), r = (tok - q.t0) * a.G + h - hk * a.G;
+    const uint32_t it0 = first + (uint32_t)(tiles - 1 - r / bm) * a.Hk + hk;
+    PaSum<JN> sum{-INFINITY, 0.f, {}};
+    for (int sp = WIDE ? grp : 0; sp < nsplit; sp += 4 * NG) {
+      float ms[4], ls[4];
+      f32x4 v[4][JN];
 #pragma unroll
-    for (int j = 0; j < JN; ++j)
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t it = it0 + (uint32_t)(sp + u * NG) * tiles * a.Hk;
+        const bool in = sp + u * NG < nsplit && it < cl.items && h < a.Hq;
+        const int64_t slot = in ? (int64_t)it * bm + r % bm : 0;
+        ms[u] = in ? cl.stat[slot * 2] : -INFINITY;
+        ls[u] = in ? cl.stat[slot * 2 + 1] : 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    if (nsplit > 1) {
-      const int tiles = (q.n * a.G + bm - 1) / bm;
-      const int hk = (int)fdiv((uint32_t)h, a.f_g), r = (tok - q.t0) * a.G + h - hk * a.G;
-      const uint32_t it0 = first + (uint32_t)(tiles - 1 - r / bm) * a.Hk + hk;
-      for (int sp = g; sp < nsplit; sp += 4 * NG) {
-        float ms[4], ls[4];
-        f32x4 v[4][JN];
+        for (int j = 0; j < JN; ++j)
+          v[u][j] = in && 64 * j + 4 * c < a.D ? *reinterpret_cast<const f32x4*>(cl.part + slot * a.Dp + 64 * j + 4 * c)
+                                               : f32x4{0.f, 0.f, 0.f, 0.f};
+      }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t it = it0 + (uint32_t)(sp + u * NG) * tiles * a.Hk;
-          ms[u] = -INFINITY;
-          ls[u] = 0.f;
-          if (sp + u * NG >= nsplit || it >= cl.items) continue;
-          const int64_t slot = (int64_t)it * bm + r % bm;
-          ms[u] = cl.stat[slot * 2];
-          ls[u] = cl.stat[slot * 2 + 1];
+      for (int u = 0; u < 4; ++u) pa_add(sum, ms[u], ls[u], v[u]);
+    }
+    const bool sees = q.len - (q.t0 + q.n - tok) >= 0;  // its position
+    S* o = (S*)a.o + (int64_t)tok * a.ost + (int64_t)h * a.osh;
+    if constexpr (!WIDE) {
+      if (h >= a.Hq) continue;
+      const float inv = pa_inv(q, sees, sum.l);
 #pragma unroll
-          for (int j = 0; j < JN; ++j)
-            if (64 * j + 4 * c < a.D) v[u][j] = *reinterpret_cast<const f32x4*>(cl.part + slot * a.Dp + 64 * j + 4 * c);
-        }
+      for (int j = 0; j < JN; ++j) {
+        const int d = 64 * j + 4 * c;
+        float* y = sum.acc[j];
+        if constexpr (JN <= 2) {  // head_dim 64 JN, aligned rows
+          if constexpr (T::kCode == AK_F32) *reinterpret_cast<f32x4*>(o + d) = f32x4{y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+          else *reinterpret_cast<u32x2*>(o + d) = u32x2{fa2_pack<T>(y[0] * inv, y[1] * inv), fa2_pack<T>(y[2] * inv, y[3] * inv)};
+        } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          if (ms[u] == -INFINITY && ls[u] == 0.f) continue;  // a slice without a key that the row sees
-          const float m_new = nan_max(m, ms[u]);
-          const float f0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-          const float f1 = ms[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ms[u] - m_new);
-          m = m_new;
-          l = l * f0 + ls[u] * f1;
-#pragma unroll
-          for (int j = 0; j < JN; ++j)
-            if (64 * j + 4 * c < a.D)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[j][e] = acc[j][e] * f0 + v[u][j][e] * f1;
+          for (int e = 0; e < 4; ++e)
+            if (d + e < a.D) o[d + e] = T::from_f(y[e] * inv);
         }
       }
-    }
-    const int me = slot_in * NG + g;
-    __syncthreads();  // the block's last rows have been read
+    } else {
+      __syncthreads();  // the unit before this one has been read
 #pragma unroll
-    for (int j = 0; j < JN; ++j)
-      if (64 * j + 4 * c < a.D)
-        *reinterpret_cast<f32x4*>(&so[me][64 * j + 4 * c]) = f32x4{acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
-    if (c == 0) {
-      sm[me] = m;
-      sl[me] = l;
-    }
-    __syncthreads();
-    if (nsplit == 1) continue;
-    float mb = -INFINITY, lb = 0.f, f[NG];
-    for (int y = 0; y < NG; ++y) mb = nan_max(mb, sm[slot_in * NG + y]);
+      for (int j = 0; j < JN; ++j)
+        *reinterpret_cast<f32x4*>(&so[grp][64 * j + 4 * c]) =
+            f32x4{sum.acc[j][0], sum.acc[j][1], sum.acc[j][2], sum.acc[j][3]};
+      if (c == 0) {
+        sm[grp] = sum.m;
+        sl[grp] = sum.l;
+      }
+      __syncthreads();
+      float mb = -INFINITY, lb = 0.f, f[NG];
+      for (int y = 0; y < NG; ++y) mb = nan_max(mb, sm[y]);
 #pragma unroll
-    for (int y = 0; y < NG; ++y) {
-      const float my = sm[slot_in * NG + y];
-      f[y] = my == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(my - mb);
-      lb += sl[slot_in * NG + y] * f[y];
-    }
-    const float inv = pa_inv(q, q.len - (q.t0 + q.n - tok) >= 0, lb);  // its position
-    S* o = (S*)a.o + (int64_t)tok * a.ost + (int64_t)h * a.osh;
-    for (int d = (wave_id() % W) * kWave + lane; d < a.D; d += W * kWave) {
-      float v = 0.f;
+      for (int y = 0; y < NG; ++y) {
+        f[y] = sm[y] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sm[y] - mb);
+        lb += sl[y] * f[y];
+      }
+      const float inv = pa_inv(q, sees, lb);
+      for (int d = threadIdx.x; d < a.D; d += kPaThreads) {
+        float v = 0.f;
 #pragma unroll
-      for (int y = 0; y < NG; ++y) v += so[slot_in * NG + y][d] * f[y];
-      o[d] = T::from_f(v * inv);
+        for (int y = 0; y < NG; ++y) v += so[y][d] * f[y];
+        o[d] = T::from_f(v * inv);
+      }
     }
   }
 }
@@ -1219,11 +1235,14 @@ static void pa_set(PaArgs& a, const PaPlan& p, void* ws) {
   a.split_rows = p.items[1] > 0 ? (int)kPaSplitRows : INT_MAX;
 }
 template <typename T, int BM0, int BM1, int JN>
-static void pa_launch_merge(const PaArgs& a, hipStream_t st) {
+static void pa_launch_merge(PaArgs& a, hipStream_t st) {
   if (a.c[0].target <= 0.f && a.c[1].target <= 0.f) return;
   const int64_t rows = (int64_t)a.s.T * a.Hq;
-  if (rows < 1024) pa_merge<T, BM0, BM1, JN, 4><<<dim3((unsigned)rows), kPaThreads, 0, st>>>(a);
-  else pa_merge<T, BM0, BM1, JN, 1><<<dim3((unsigned)std::min<int64_t>(cdiv(rows, kPaWaves), 2048)), kPaThreads, 0, st>>>(a);
+  // 64 tokens of 32 heads, up to 7 slices: the whole call 129.6 us with a group per row, 132.0 with a block
+  const bool wide = rows < 1024;
+  a.f_units = make_fastdiv((uint32_t)(wide ? a.Hq : (a.Hq + 3) / 4));
+  if (wide) pa_merge<T, BM0, BM1, JN, true><<<dim3((unsigned)rows), kPaThreads, 0, st>>>(a);
+  else pa_merge<T, BM0, BM1, JN, false><<<dim3((unsigned)std::min<int64_t>(cdiv(rows, 4 * kPaWaves), 2048)), kPaThreads, 0, st>>>(a);
 }
 template <typename T>
 static int launch_general(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
@@ -1307,7 +1326,6 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
   a.c_log2 = sm_scale * kFaLog2e;
   a.f_g = make_fastdiv((uint32_t)a.G);
   a.f_hk = make_fastdiv((uint32_t)a.Hk);
-  a.f_hq = make_fastdiv((uint32_t)a.Hq);
   a.s = make_paged(page_table, q_starts, kv_lens, T, B, num_pages, page_size, max_pages, table_stride);
   // K rows in 16-byte vectors
   const int vw = dtype == AK_F32 ? 4 : 8;
