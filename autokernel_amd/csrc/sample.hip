@@ -291,8 +291,8 @@ __device__ __forceinline__ uint64_t sm_last(SampleShared& sh, const SampleSums<P
   __syncthreads();
   return sh.found[1];
 }
-// About how many elements the bins up to `at` hold: counted, or their masses over the weight in a bin's middle.
-__device__ __forceinline__ uint32_t sm_upto(SampleShared& sh, const SampleSums<kBinsPer>& s, int at, bool counts) {
+// About how many elements the bins up to `at` hold: their masses over the weight in a bin's middle.
+__device__ __forceinline__ uint32_t sm_upto(SampleShared& sh, const SampleSums<kBinsPer>& s, int at) {
   __syncthreads();
   if (threadIdx.x == 0) sh.n = 0;
   __syncthreads();
@@ -302,7 +302,7 @@ __device__ __forceinline__ uint32_t sm_upto(SampleShared& sh, const SampleSums<k
   for (int i = 0; i < kBinsPer; ++i) {
     const int b = threadIdx.x * kBinsPer + i;
     const float in = (float)(s.upto[i] - before);
-    if (b <= at) n += counts ? in : in * __builtin_amdgcn_exp2f(((float)b + 0.5f) * (kSpan / kBins) - 42.0f);
+    if (b <= at) n += in * __builtin_amdgcn_exp2f(((float)b + 0.5f) * (kSpan / kBins) - 42.0f);
     before = s.upto[i];
   }
   n = wave_sum(n);
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
     }
     if (step == 1 && !(top_p < 1.0f)) continue;
     const uint64_t target = step == 0   ? min((uint64_t)top_k, z)  // a row with fewer elements ends at its last one
-                            : step == 1 ? max((uint64_t)__builtin_ceil((double)top_p * (double)z), (uint64_t)1)
+                            : step == 1 ? max((uint64_t)__builtin_ceil((double)fmaxf(top_p, 0.f) * (double)z), (uint64_t)1)
                                         : (uint64_t)((double)u * (double)z) + 1;
     uint64_t before = 0;
     if (!listed) {
@@ -582,7 +582,7 @@ __global__ __launch_bounds__(kSmThreads) void sample_rows(const SampleArgs a) {
       uint64_t lo = sm_pair(sm_first(r, (float)bin.at), INT_MAX), hi = most;
       const uint64_t end = sm_pair(r.low, r.low_last);
       if (lo < end) lo = end;
-      if (step > 0 && sm_upto(sh, s, bin.at, counts) <= kRanked) {
+      if (step > 0 && sm_upto(sh, s, bin.at) <= kRanked) {
         sm_gather<T>(sh, r, x, V, lo, hi);
         listed = sh.n <= kList;
       }

@@ -7,8 +7,8 @@ falling order (equal logits: lowest index first), each step on what the one befo
   top_k  keeps the first top_k (0: all)
   top_p  keeps the shortest prefix whose mass reaches top_p of theirs (1: all; one element at least)
 and the token is the first element whose running mass exceeds u times the mass kept. temperature 0 is
-greedy: the maximum, lowest index; others count as 1e-20 at least. Every setting is a number or a tensor with one value per row
-(float32; top_k int32).
+greedy: the maximum, lowest index; others count as 1e-20 at least. Every setting is a number or a tensor with one
+value per row (float32; top_k int32), where a value below its range counts as 0, top_p and min_p above 1 as 1.
 
 The random numbers are the caller's, so a seed gives the same tokens whatever the batch; weights and sums
 are exact to better than 2^-40 and add up in no particular order, so a row and its number always give the

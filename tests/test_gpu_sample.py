@@ -180,6 +180,25 @@ def test_numbers_outside_their_range(gpu):
         assert torch.equal(sample(x, u, **kw), sample(x, same, **kw))
 
 
+@pytest.mark.parametrize("V", [40, 5000])
+def test_settings_outside_their_range(gpu, V):
+    """In a tensor, values below the range count as 0 and top_p, min_p above 1 as 1."""
+    x, u = zipf(6, V, torch.float32, 5)
+
+    def rows(*v, dtype=torch.float32):
+        return torch.tensor(v, dtype=dtype, device="cuda")
+    inf = float("inf")
+    low, high = rows(-0.5, -1e-30, -3.0, -1e30, -inf, -0.0), rows(1.0, 1.5, 1e30, inf, 2.0, 1.0)
+    one, zero = torch.ones_like(u), torch.zeros_like(u)
+    assert torch.equal(sample(x, u, top_p=low), sample(x, u, top_k=1))
+    assert torch.equal(sample(x, u, top_p=low, top_k=30), sample(x, u, top_k=1))
+    assert torch.equal(sample(x, u, top_p=high), sample(x, u, top_p=one))
+    assert torch.equal(sample(x, u, min_p=low), sample(x, u, min_p=zero))
+    assert torch.equal(sample(x, u, min_p=high), sample(x, u, min_p=one))
+    k = rows(-1, -(1 << 31), 0, V, V + 1, (1 << 31) - 1, dtype=torch.int32)
+    assert torch.equal(sample(x, u, top_k=k), sample(x, u))
+
+
 @pytest.mark.parametrize("dt", DT)
 def test_strides_and_shapes(gpu, dt):
     x, u = zipf(6, 1003, dt, 8)
