@@ -231,6 +231,8 @@ extern "C" int ak_kv_append(int dtype, const void* q, const void* k, const void*
       (Hkv > 0 && (!k || !v || !k_strides || !v_strides || !k_cache_strides || !v_cache_strides)) ||
       (Hkv > 0 && num_pages > 0 && (!k_cache || !v_cache)))
     return AK_EINVAL;
+  for (int i = 0; i < 3; ++i)
+    if (Hkv > 0 && (k_cache_strides[i] < 0 || v_cache_strides[i] < 0)) return AK_EINVAL;
   AppendArgs a{};
   a.q = q, a.k = k, a.v = v, a.qo = q_out, a.kc = k_cache, a.vc = v_cache;
   a.ct = turn ? cos_t : nullptr, a.st = turn ? sin_t : nullptr;

@@ -115,9 +115,7 @@ __device__ __forceinline__ int pa_chunk(const PaArgs& a, const PaBatch& x) {
   const float c = ceilf(w / a.c[CLS].target / (float)kPaSlice) * (float)kPaSlice;
   return pa_uniform(c >= 1e9f ? INT_MAX : max((int)c, kPaSlice));
 }
-__device__ __forceinline__ int pa_splits(int len, int chunk) {
-  return chunk == INT_MAX ? 1 : max(1, (len + chunk - 1) / chunk);
-}
+__device__ __forceinline__ int pa_splits(int len, int chunk) { return len > 0 ? (len - 1) / chunk + 1 : 1; }
 
 // Item `it` of a class; false when there are fewer. Within a sequence the KV heads run fastest (one
 // per XCD, whose L2 then serves the tiles that share a head's keys), then tiles, last rows first (they see
@@ -229,7 +227,13 @@ __device__ void pa_row(const PaArgs& a, int b, int hk, const typename T::S* qrow
   }
 }
 
-// Row r of a tile: its output row, and the end of the keys that it sees in [.., hi).
+// Where an item's keys begin, and where those of them end that lie below `seen` (without passing 2^31 on the way).
+__device__ __forceinline__ int pa_begin(const PaItem& it) { return pa_uniform(it.split ? it.split * it.chunk : 0); }
+__device__ __forceinline__ int pa_end(const PaItem& it, int seen) {
+  const int lo = pa_begin(it);
+  return pa_uniform(lo + min(seen - lo, it.chunk));
+}
+// Row r of a tile: the end of the keys that it sees.
 __device__ __forceinline__ int pa_seen(const PaItem& it, int r, FastDiv f_g) {
   return max(0, it.seq.len - it.seq.n + (int)fdiv((uint32_t)r, f_g) + 1);
 }
@@ -277,9 +281,8 @@ template <typename T>
 __global__ __launch_bounds__(kPaThreads) void pa_general(const PaArgs a) {
   PaItem it;
   if (!pa_find<kPaRowTile, 0>(a, blockIdx.x, it)) return;
-  const int r0 = it.tile * kPaRowTile, lo = it.nsplit == 1 ? 0 : it.split * it.chunk;
-  pa_one_by_one<T, kPaRowTile, 0>(a, it, r0, min(it.seq.n * a.G, r0 + kPaRowTile), lo,
-                                  it.nsplit == 1 ? INT_MAX : lo + it.chunk);
+  const int r0 = it.tile * kPaRowTile;
+  pa_one_by_one<T, kPaRowTile, 0>(a, it, r0, min(it.seq.n * a.G, r0 + kPaRowTile), pa_begin(it), pa_end(it, it.seq.len));
 }
 
 // Sliced rows: the partials of each (row, query head), added in slice order by groups of 16 lanes (lane c: dims
@@ -561,8 +564,7 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
     for (int s = 0; s < NS; ++s) qf[s] = r < rows ? ld16(q + s * 32 + g * 8) : u32x4{0u, 0u, 0u, 0u};
   }
   const int rl = min(rows, r0 + kPrRows) - 1;  // the tile's last row sees the most
-  const int kbeg = pa_uniform(it.nsplit == 1 ? 0 : it.split * it.chunk);
-  const int kend = pa_uniform(min(pa_seen(it, rl, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk));
+  const int kbeg = pa_begin(it), kend = pa_end(it, pa_seen(it, rl, a.f_g));
   const int full = pa_uniform(pa_seen(it, r0, a.f_g));  // every row sees the keys below
 
   struct Pages {
@@ -716,8 +718,7 @@ __device__ __forceinline__ void pa_rows_f32_item(const PaArgs& a, uint32_t item,
       qf[s] = r < rows ? *reinterpret_cast<const f32x4*>(q + 4 * s) : f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const int rl = min(rows, r0 + kPrRows) - 1;
-  const int kbeg = pa_uniform(it.nsplit == 1 ? 0 : it.split * it.chunk);
-  const int kend = pa_uniform(min(pa_seen(it, rl, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk));
+  const int kbeg = pa_begin(it), kend = pa_end(it, pa_seen(it, rl, a.f_g));
   const int full = pa_uniform(pa_seen(it, r0, a.f_g));
   struct Pages {
     int k, v[NV];
@@ -863,9 +864,7 @@ __device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, Pt
   const int w = __builtin_amdgcn_readfirstlane(wave_id());
   const int rows = it.seq.n * a.G, r0 = it.tile * kPtRows, rw0 = r0 + 32 * w;  // this wave's first row
   const int my_r = rw0 + l32;
-  const int kbeg = pa_uniform(it.nsplit == 1 ? 0 : it.split * it.chunk);
-  const int kend = pa_uniform(
-      min(pa_seen(it, min(rows, r0 + kPtRows) - 1, a.f_g), it.nsplit == 1 ? INT_MAX : kbeg + it.chunk));
+  const int kbeg = pa_begin(it), kend = pa_end(it, pa_seen(it, min(rows, r0 + kPtRows) - 1, a.f_g));
   const int tk = (int)fdiv((uint32_t)min(my_r, rows - 1), a.f_g);
   const int64_t head = it.hk * a.G + min(my_r, rows - 1) - tk * a.G, tok = it.seq.t0 + tk;
   const int nt = pa_uniform((max(kend - kbeg, 0) + kFaBKV - 1) / kFaBKV);
@@ -1314,7 +1313,9 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
   if (T == 0 || B == 0 || Hq == 0) return AK_OK;
   if (!q || !o || !q_strides || !o_strides || !k_cache_strides || !v_cache_strides) return AK_EINVAL;
   if (num_pages > 0 && (!k_cache || !v_cache)) return AK_EINVAL;
-  if (!(sm_scale > 0.f) || sm_scale > 3e38f) return AK_EINVAL;
+  if (!(sm_scale > 0.f) || sm_scale > 2e38f) return AK_EINVAL;  // (log2(e) times it is finite)
+  for (int i = 0; i < 3; ++i)
+    if (k_cache_strides[i] < 0 || v_cache_strides[i] < 0) return AK_EINVAL;
   const int64_t need = ak_paged_attn_workspace_bytes(dtype, T, B, Hq, Hkv, D, page_size, max_pages);
   if (need > 0 && (!host_aligned16(workspace) || !workspace || workspace_bytes < need)) return AK_EINVAL;
   PaArgs a{};
@@ -1339,7 +1340,7 @@ extern "C" int ak_paged_attn(int dtype, const void* q, const void* k_cache, cons
   for (const int64_t x : {a.kct, a.vct})
     if (x < D || x > (1 << 24) || x * page_size >= (int64_t)1 << 31) fast = false;
   for (const int64_t x : {a.kcp, a.vcp})
-    if (x < 0 || x >= (int64_t)1 << 31) fast = false;
+    if (x >= (int64_t)1 << 31) fast = false;
   const PaPlan p = pa_plan(dtype, T, B, Hq, Hkv, D, page_size, max_pages, fast);
   if (!pa_plan_fits(p)) return AK_EINVAL;
   AK_DISPATCH(dtype, T_, {

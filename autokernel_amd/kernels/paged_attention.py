@@ -31,8 +31,8 @@ def kernel_fn(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
     if q.shape[1] % k_cache.shape[1]:
         raise ValueError(f"paged_attention: {q.shape[1]} query heads not a multiple of {k_cache.shape[1]} KV heads")
     scale = float(q.shape[2] ** -0.5 if sm_scale is None else sm_scale)
-    if not 0.0 < scale < 3e38:
-        raise ValueError(f"paged_attention: sm_scale {scale} must be positive and finite")
+    if not 0.0 < scale <= 2e38:
+        raise ValueError(f"paged_attention: sm_scale {scale} must be above 0, at most 2e38")
     if out is None:
         out = q.new_empty(q.shape)
     elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device

@@ -334,7 +334,8 @@ int ak_flash_attn_fwd_ws(int dtype, const void* Q, const void* K, const void* V,
 /*
  * The paged cache of ak_kv_append and ak_paged_attn. K and V each live in num_pages pages of page_size
  * slots, every slot one token's [Hkv, D]; element strides (page, head, slot) say how a page is laid out
- * ([pages, Hkv, page_size, D] and [pages, page_size, Hkv, D] alike), the last dim is contiguous.
+ * ([pages, Hkv, page_size, D] and [pages, page_size, Hkv, D] alike; none negative), the last dim is
+ * contiguous.
  * A call's T rows are the sequences' new tokens one after another: sequence b has rows
  * q_starts[b] .. q_starts[b + 1] - 1 (q_starts: int32 [B + 1], rising) and, these new tokens included,
  * kv_lens[b] cached tokens (int32 [B]). So row t is at position kv_lens[b] - (q_starts[b + 1] - t), and
@@ -367,7 +368,8 @@ int ak_kv_append(int dtype, const void* q, const void* k, const void* v, void* q
 /*
  * Attention of the new tokens over the paged cache: O_t = softmax_j(q_t . K_j * sm_scale) V_j over the
  * positions j up to row t's own (the new tokens' K and V are in the cache already, see ak_kv_append).
- * q, o: [T, Hq, D] by (row, head) strides; query head h reads KV head h / (Hq / Hkv). sm_scale > 0.
+ * q, o: [T, Hq, D] by (row, head) strides; query head h reads KV head h / (Hq / Hkv). sm_scale from above 0 to
+ * 2e38. T * Hq below 2^31, and few enough tiles of rows for one grid (AK_EINVAL otherwise).
  * Any mix of single tokens and chunks. fp32 scores, softmax statistics and sums. What a row does not see
  * (later tokens, slots past the sequence's end, infinities and NaN among them) has no influence on it.
  * A row that sees nothing (position below zero) is zero. A row that sees a position whose page is not in
@@ -393,10 +395,12 @@ int ak_paged_attn(int dtype, const void* q, const void* k_cache, const void* v_c
  * index first), each step on what the one before has left:
  *   min-p: w_i >= min_p (min_p <= 0: all; above 1: as 1)
  *   top-k: the first top_k (top_k <= 0: all)
- *   top-p: the shortest prefix whose mass reaches top_p of theirs, one element at least (top_p >= 1: all)
+ *   top-p: the shortest prefix whose mass reaches top_p of theirs, one element at least (top_p >= 1: all;
+ *     below 0: as 0)
  *   the token: the first element whose running mass exceeds u times the mass kept
- * temperature 0 takes the maximum (lowest index); others count as 1e-20 at least, and 1e30 is the highest. u: fp32 [rows], taken as 0 below 0 and
- * as 1 - 2^-24 above it. Each setting is a scalar, or an array with one value per row where its _rows pointer is not NULL.
+ * temperature 0 takes the maximum (lowest index); others count as 1e-20 at least, and 1e30 is the highest.
+ * u: fp32 [rows], taken as 0 below 0 and as 1 - 2^-24 above it. Each setting is a scalar, or an array with one
+ * value per row where its _rows pointer is not NULL.
  * tokens: int64 [rows]; -1 for a row that holds a NaN, one whose maximum is -infinity and one with a setting
  * from an array that is a NaN or, for the temperature, outside 0 .. 1e30 (as scalars: AK_EINVAL).
  * +infinity counts as the largest finite float. Weights and their sums are exact to better than 2^-40

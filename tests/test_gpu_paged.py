@@ -1,6 +1,8 @@
 """kv_append and paged_attention against a 64-bit restatement (paged_oracle.py), on the GPU."""
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -204,6 +206,26 @@ def test_attention_cache_past_32_bits(gpu):
     want, tol = po.attention(b)
     out = attn(b.dev(b.q), kc, vc, table.cuda(), b.starts.cuda(), b.lens_t.cuda()).double().cpu()
     assert ((out - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("width", [524256, 524287])  # of 2^31 / 4096: the tiled kernel's longest cache; beyond, the general one's
+def test_attention_positions_up_to_2_31(gpu, width):
+    """Nearly 2^31 cached tokens: one page over and over (scores 0, values 1) and a last one with scores of 13.125 and
+    values of -1, which carries half of the weight. Sums of ones are exact to 2^24, and what is added up of slices
+    and exponentials rounds a few thousand times at 2^-24: below 1e-3 / 4 with the share of bf16 weights (2^-8 of
+    the last slice's 1 / 1500)."""
+    page, D = 4096, 64
+    kc = torch.zeros(2, 1, page, D, dtype=BF16, device="cuda")
+    vc = torch.ones_like(kc)
+    kc[1], vc[1] = 1.640625, -1.0
+    table = torch.zeros(1, width, dtype=torch.int32, device="cuda")
+    table[0, -1] = 1
+    n = width * page
+    starts, lens = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([0, 1], [n]))
+    out = attn(torch.ones(1, 1, D, dtype=BF16, device="cuda"), kc, vc, table, starts, lens).double().cpu()
+    last = page * math.exp(8 * 1.640625)
+    want = (n - page - last) / (n - page + last)
+    assert (out - want).abs().max() <= 2.0 ** -8 * abs(want) + 2.5e-4, (out.flatten()[0], want)
 
 
 def test_attention_streams_and_repeats(gpu):

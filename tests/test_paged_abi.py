@@ -30,6 +30,7 @@ def test_paged_attention_refusals(lib):
                 dict(starts=None), dict(lens=None), dict(qs=None), dict(os=None), dict(ks=None), dict(vs=None),
                 dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(T=1 << 31),
                 dict(pages=1 << 31), dict(page=1 << 20, width=1 << 12, stride=1 << 12), dict(Hq=1 << 20, Hkv=1),
+                dict(scale=2.1e38), dict(ks=_lib.i64_array([64, -64, 64])), dict(vs=_lib.i64_array([-1, 64, 64])),
                 dict(width=400, stride=400),                                # needs a workspace
                 dict(width=400, stride=400, ws=ctypes.c_void_p(8), wsb=1 << 40)):  # misaligned
         assert call(**bad) == _lib.AK_EINVAL, bad
@@ -55,6 +56,7 @@ def test_kv_append_refusals(lib):
     for bad in (dict(dtype=7), dict(T=-1), dict(B=-1), dict(Hq=-1), dict(D=0), dict(rot=63), dict(rot=66), dict(rot=-2),
                 dict(rows=-1), dict(page=0), dict(stride=3), dict(q=None), dict(k=None), dict(v=None), dict(qo=None),
                 dict(kc=None), dict(vc=None), dict(cos=None), dict(sin=None), dict(rot=0), dict(qs=None), dict(kcs=None),
+                dict(kcs=_lib.i64_array([64, 64, -64])), dict(vcs=_lib.i64_array([-64, 64, 64])),
                 dict(table=None), dict(starts=None), dict(lens=None), dict(T=1 << 31), dict(Hkv=1 << 20)):
         assert call(**bad) == _lib.AK_EINVAL, bad
     assert call(D=258) == _lib.AK_EUNSUPPORTED
