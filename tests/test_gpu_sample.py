@@ -172,6 +172,44 @@ def test_rows_without_a_token(gpu, dt):
             assert got[7] == -1 and got[8] >= 0 and got[6] >= 0
 
 
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("V", [65535, 65536, 65537, 131072, 200001])
+def test_long_runs_of_equal_values(gpu, dt, V):
+    """Values that fill most of a row, around and past what 16 bits count: a constant, a masked row whose mask is a
+    small number, the lowest finite one or -inf, two values in turn, neighbours in falling order."""
+    g = torch.Generator().manual_seed(V)
+    rows = []
+    for fill in (0.0, 2.5, -3.0, torch.finfo(dt).min, -float("inf"), torch.finfo(dt).max):
+        row = torch.full((V,), fill)
+        rows.append(row.clone())
+        at = torch.randperm(V, generator=g)[:300]
+        row[at] = torch.randn(300, generator=g) * 2
+        rows.append(row)
+    rows.append((torch.arange(V) % 2).float())
+    rows.append(torch.where(torch.arange(V) < 70000, -0.0, 0.0))
+    x = torch.stack(rows).to(dt).cuda()
+    u = torch.rand(len(x), generator=g).cuda()
+    check(x, u, f"runs of {V}")
+    check(x, u, f"runs of {V}", top_p=0.37)
+    check(x, u, f"runs of {V}", top_k=1000, min_p=0.01)
+    check(x, u, f"runs of {V}", temperature=torch.rand(len(x), generator=g).cuda() * 2 + 0.1, top_k=70000)
+    check(x, u, f"runs of {V}", temperature=0.0)
+
+
+@pytest.mark.parametrize("dt", DT)
+def test_signed_zeros_are_equal(gpu, dt):
+    x = torch.full((16, 300), -50.0)
+    x[:, 40::7] = 0.0
+    x[:, 43::14] = -0.0
+    x[8:, 5] = -0.0
+    n = int((x[0] == 0).sum())
+    x, u = x.to(dt).cuda(), ((torch.arange(16) + 0.5) / 16).cuda()
+    check(x, u, "zeros")
+    check(x, u, "zeros", top_k=n // 2)
+    check(x, u, "zeros", top_p=0.31)
+    check(x, u, "zeros", temperature=0.0)
+
+
 def test_numbers_outside_their_range(gpu):
     x, _ = zipf(6, 500, torch.float32, 4)
     u = torch.tensor([-1.0, float("nan"), 1.0, 7.0, float("inf"), -float("inf")], device="cuda")
