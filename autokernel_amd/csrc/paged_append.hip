@@ -7,6 +7,8 @@
 // once; a decode step's few tokens by the launch. A wave takes 16-byte vectors of one token's heads (q,
 // then k, then v). Its lanes keep one column each, so a lane reads its table entries once for all heads;
 // the page comes from one table read per wave. Few tokens are spread over more waves per token.
+// 8000 tokens of prompts (32 + 2 x 8 heads of 128, bf16): 196 MB in 35 us, 5.6 TB/s (a large copy 5.1); 48 tokens: 4 us,
+// the launch and the chain of lengths, page number and row.
 #include <limits.h>
 
 #include <algorithm>
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(kApWaves* kWave) void append_vec(const AppendArgs a
   }
 }
 
-// Any alignment: a wave walks its token's heads one pair or one unturned element per lane.
+// Any alignment, element by element: a wave walks its token's heads one pair or one unturned element per lane.
 template <typename T, bool HALVES>
 __global__ __launch_bounds__(kApWaves* kWave) void append_scalar(const AppendArgs a) {
   using S = typename T::S;

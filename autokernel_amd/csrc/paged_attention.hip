@@ -275,7 +275,8 @@ __device__ void pa_one_by_one(const PaArgs& a, const PaItem& it, int r_begin, in
   }
 }
 
-// Any type, head_dim and alignment: one wave per row, four rows per block.
+// Any type, head_dim and alignment: one wave per row, four rows per block. Each row reads its keys for itself, from the
+// L2 where rows share them (64 ragged sequences of 200 to 8000 tokens: 1391 us, 130 by pa_rows).
 constexpr int kPaRowTile = kPaWaves;
 template <typename T>
 __global__ __launch_bounds__(kPaThreads) void pa_general(const PaArgs a) {
@@ -290,6 +291,8 @@ __global__ __launch_bounds__(kPaThreads) void pa_general(const PaArgs a) {
 // itself (WIDE false: a wave takes four heads of one token); with few, the block's sixteen groups share a row,
 // so that 64 slices' partials are in flight at once, and combine in group order. The grid is bounded and walks the
 // rows: in most calls with many rows nothing is sliced and it ends at once.
+// Bound by reading the partials where there are many: 512 tokens of 32 heads in 4 slices, 35 MB, 9.5 us (a wave per
+// row 16); by latency otherwise, 4.4 to 8 us.
 template <int JN>
 struct PaSum {
   float m, l, acc[JN][4];  // exp2 base, sum, weighted values
@@ -445,6 +448,9 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
 //   * Weights are rounded to the element type for the product; the sum adds the rounded ones.
 // Keys past a row's position weigh nothing as long as their V is finite. Where a result is NaN, or a page
 // lies outside the cache, the rows are computed again by pa_row.
+// 64 sequences of 200 to 8000 cached tokens, one new one each, 8 KV heads of 128 in bf16: 613 MB in 120 us, 5.1 TB/s (a
+// large copy moves as much), and 7.5 for the merge. One sequence of 1000: 14.4 us, eight CUs' latency: 1 us to find
+// the item, 2 to its page numbers and 3 per two steps of keys.
 constexpr int kPrRows = 16, kPrKeys = 32;
 struct PrMaximum {
   __device__ __forceinline__ float operator()(float a, float b) const { return fa2_max(a, b); }
@@ -695,6 +701,7 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
 // a quarter of one key's row: the contraction's order is free, so k index g of step s is dim g D / 4 + s and K
 // and Q load as whole vectors. S^T leaves lane group g with the scores of keys 4 g .. 4 g + 3, so step t of
 // O^T += V^T P^T takes keys 4 g + t: weight t as it stands, and the V rows of four consecutive keys.
+// 43 tokens of four sequences over 4000 cached ones, 12 heads of 64 on 4 KV heads: 16.5 us a call, 84 by pa_general.
 template <int D, int PG, int NW>
 __device__ __forceinline__ void pa_rows_f32_item(const PaArgs& a, uint32_t item, PrShared<D, NW>& sh) {
   constexpr int NS = D / 4, VW = D / 16;
@@ -831,7 +838,9 @@ __device__ __forceinline__ void pa_rows_f32_item(const PaArgs& a, uint32_t item,
 //     rest arrives as zeros). The resources of 64 tiles are made at once, one per lane.
 //   * No pass over what a row does not see: V of masked keys only has to be finite. Where a row's result is
 //     NaN, or a page lies outside the cache, the item's rows are computed again by pa_row.
-// Bound by the MFMA and the softmax VALU work, as fa_fwd2 is.
+// Bound by the MFMA and the softmax VALU work, as fa_fwd2 is. 512 tokens after 16001 (32 heads of 128, 8 KV heads,
+// bf16): 156 us, 875 TFLOP/s, MFMA busy 41 % of the time, half of it waiting; four prompts of 2048: 167 to 186 us, 740
+// to 820. A prompt of 8192 runs at 992 TFLOP/s, fa_fwd2 on dense keys at 1074.
 constexpr int kPtRows = 32 * kPaWaves;
 
 // fa2_dma16 for a resource made right before it: its words come from v_readlane / v_readfirstlane, and a vector
@@ -1189,8 +1198,19 @@ __global__ __launch_bounds__(kPaThreads, 2) void pa_mixed(const PaArgs a) {
 }
 
 // What a call launches: the most items of each class and their partials. Keys are sliced only where some
-// sequence can be longer than kPaMinSliced, below which the merge costs more than the shorter walk saves.
-constexpr int64_t kPaSplitRows = 64, kPaMinSliced = 1536;
+// sequence can be longer than kPaMinSliced, below which the merge costs what the shorter walk saves (one
+// sequence of 1000 keys: 5 us each).
+// Items aimed at: 1536 tiles of 16 rows (64 ragged sequences 128.6 us; 512: 135.8, 1024: 131, 2048: 131.4), 512 of 128
+// rows (512 tokens after 16001 157 us; 1024: 172).
+// A sequence of more rows than one tile of 16 takes tiles of 128, which read its keys once (64 sequences over 2000
+// tokens, 32 / 64 rows each: 103 / 109 us, in tiles of 16: 179 / 204), in calls where that pays:
+//   * With sliced keys, where some sequence has several new tokens (two of 8 over 8000: 24.4 us, 28.6 without), or with
+//     more than kPaTiledRows rows. The rows of up to 16 single tokens stay with blocks of eight waves (8 / 16
+//     sequences of 1000, 4 rows each: 15.7 / 17.4 us, 19.4 / 21.1 beside empty large tiles).
+//   * With whole keys, where the tiles of 16 would be more than two per CU, about what runs at a time: a wave of the
+//     large tiles walks all the keys, a wave of the small ones a fourth (30 tokens each of 4 sequences of 1000: 17.7 us,
+//     31.8 with the large tiles; 100 tokens each: 32.3, 44.0 without).
+constexpr int64_t kPaSplitRows = 16, kPaTiledRows = 64, kPaMinSliced = 1536, kPaOneEach = 256;
 struct PaPlan {
   int bm0;
   int64_t items[2], target[2], ws[2];  // ws: floats of a class's partials
@@ -1201,14 +1221,16 @@ static PaPlan pa_plan(int dtype, int64_t T, int64_t B, int64_t Hq, int64_t Hk, i
                       int64_t width, bool fast) {
   PaPlan p{};
   const int64_t keys = page_size * width, G = Hq / Hk, rows = T * G, seqs = std::min(B, T);
-  const bool tiles = fast && dtype != AK_F32 && page_size % 16 == 0 && rows > kPaSplitRows;
+  const bool sliced = keys > kPaMinSliced;
   p.bm0 = fast ? kPrRows : kPaRowTile;
   p.items[0] = (rows / p.bm0 + seqs) * Hk;
+  const bool tiles = fast && dtype != AK_F32 && page_size % 16 == 0 && rows > kPaSplitRows &&
+                     (sliced ? T > B || rows > kPaTiledRows : (rows / kPrRows + seqs / 2) * Hk > 2 * kPaOneEach);
   if (tiles) {
-    p.items[0] = std::min(p.items[0], seqs * (kPaSplitRows / p.bm0) * Hk);
+    p.items[0] = std::min(p.items[0], seqs * ((kPaSplitRows + p.bm0 - 1) / p.bm0) * Hk);
     p.items[1] = (rows / kPtRows + std::min(seqs, rows / (kPaSplitRows + 1))) * Hk;
   }
-  if (keys > kPaMinSliced) {
+  if (sliced) {
     p.target[0] = 1536;
     // two tiles per CU at a time; four times that many are work enough unsliced
     if (tiles && rows / kPtRows * Hk < 4 * 512) p.target[1] = 512;
@@ -1240,8 +1262,11 @@ static void pa_launch_merge(PaArgs& a, hipStream_t st) {
   // 64 tokens of 32 heads, up to 7 slices: the whole call 129.6 us with a group per row, 132.0 with a block
   const bool wide = rows < 1024;
   a.f_units = make_fastdiv((uint32_t)(wide ? a.Hq : (a.Hq + 3) / 4));
+  // where only sequences with few rows may be sliced, blocks for as many rows as these can have
+  const int64_t most = a.c[1].target > 0.f || a.c[1].items == 0 ? rows : (int64_t)a.s.B * a.split_rows * a.Hk;
+  const int64_t blocks = std::min<int64_t>(cdiv(std::min(rows, most), 4 * kPaWaves), 2048);
   if (wide) pa_merge<T, BM0, BM1, JN, true><<<dim3((unsigned)rows), kPaThreads, 0, st>>>(a);
-  else pa_merge<T, BM0, BM1, JN, false><<<dim3((unsigned)std::min<int64_t>(cdiv(rows, 4 * kPaWaves), 2048)), kPaThreads, 0, st>>>(a);
+  else pa_merge<T, BM0, BM1, JN, false><<<dim3((unsigned)blocks), kPaThreads, 0, st>>>(a);
 }
 template <typename T>
 static int launch_general(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
@@ -1250,11 +1275,12 @@ static int launch_general(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
   pa_launch_merge<T, kPaRowTile, kPaRowTile, 4>(a, st);
   return record_launch();
 }
-// Blocks of eight waves where a batch has at most one per CU: each wave walks half as many keys.
+// Blocks of eight waves where a batch has at most one per CU: each wave walks half as many keys (one sequence of
+// 1000: 14.4 us, 15.8 with four). With more blocks than that four waves share a CU with three other blocks.
 template <typename T, int D, int PG>
 static void launch_rows(const PaArgs& a, const PaPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)p.items[0]);
-  if (p.items[0] <= 256) pa_rows<T, D, PG, 8><<<grid, 8 * kWave, 0, st>>>(a);
+  if (p.items[0] <= kPaOneEach) pa_rows<T, D, PG, 8><<<grid, 8 * kWave, 0, st>>>(a);
   else pa_rows<T, D, PG, kPaWaves><<<grid, kPaThreads, 0, st>>>(a);
 }
 template <typename T, int D>

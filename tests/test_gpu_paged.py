@@ -34,22 +34,34 @@ def _check_attn(b, what="", scale=None, **kw):
     return out
 
 
+# Page tables for more than 1536 tokens (whatever the sequences hold): keys are sliced, and sequences of more than 16 rows
+# per KV head take the large tiles.
+LONG = pytest.mark.parametrize("long", [False, True])
+
+
+def _slack(long, page):
+    return 1600 // page + 1 if long else 1
+
+
 SHAPES = [(8, 2, 128), (4, 4, 64), (6, 2, 64), (32, 2, 128), (3, 1, 80), (5, 5, 17), (4, 2, 256), (16, 1, 128), (2, 1, 1)]
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("heads,kv_heads,D", SHAPES)
-def test_attention_shapes(gpu, dtype, heads, kv_heads, D):
+@LONG
+def test_attention_shapes(gpu, dtype, heads, kv_heads, D, long):
     # single tokens, chunks, an empty sequence, one whose tokens are all new, a length of one
-    b = po.Batch([1, 5, 0, 37, 1, 2], [1, 70, 0, 37, 300, 3], heads, kv_heads, D, 16, dtype, seed=D, pad=3)
+    b = po.Batch([1, 5, 0, 37, 1, 2], [1, 70, 0, 37, 300, 3], heads, kv_heads, D, 16, dtype, seed=D, pad=3,
+                 slack=_slack(long, 16))
     _check_attn(b, "shapes")
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 24, 48, 64, 100, 1024])
 @pytest.mark.parametrize("layout", ["hnd", "nhd"])
-def test_attention_page_sizes(gpu, dtype, page, layout):
-    b = po.Batch([70, 1, 9], [129, 257, 64], 4, 2, 64, page, dtype, seed=page, layout=layout)
+@LONG
+def test_attention_page_sizes(gpu, dtype, page, layout, long):
+    b = po.Batch([70, 1, 9], [129, 257, 64], 4, 2, 64, page, dtype, seed=page, layout=layout, slack=_slack(long, page))
     _check_attn(b, f"page {page} {layout}")
 
 
@@ -63,8 +75,32 @@ def test_attention_unaligned(gpu, dtype, shift, layout):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("n,L", [(1, 1), (1, 2), (1, 63), (1, 64), (1, 65), (2, 64), (63, 63), (64, 64), (65, 65), (33, 127),
                                  (17, 128), (129, 129), (130, 400), (1, 255), (1, 256), (1, 257), (1, 511), (3, 513)])
-def test_attention_lengths(gpu, dtype, n, L):
-    _check_attn(po.Batch([n], [L], 8, 2, 128, 16, dtype, seed=L), "lengths")
+@LONG
+def test_attention_lengths(gpu, dtype, n, L, long):
+    _check_attn(po.Batch([n], [L], 8, 2, 128, 16, dtype, seed=L, slack=_slack(long, 16)), "lengths")
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,D,page", [(32, 4, 128, 16), (16, 16, 64, 48)])
+def test_attention_large_tiles_unsliced(gpu, dtype, heads, kv_heads, D, page):
+    """Rows enough for the large tiles over short tables; among them rows whose masked values are not finite, and a page
+    outside the cache."""
+    b = po.Batch([600, 1, 17, 130], [900, 40, 33, 129], heads, kv_heads, D, page, dtype, seed=D, lead=1, pad=2)
+    _check_attn(b, "large tiles")
+    last = int(b.table[0, 899 // page])
+    b.vc[last, :, 899 % page] = float("nan")
+    b.kc[last, :, 899 % page] = float("inf")
+    b.table[3, 0] = b.pages
+    want, tol = po.attention(po.Batch([600, 1, 17, 130], [900, 40, 33, 129], heads, kv_heads, D, page, dtype, seed=D, lead=1,
+                                      pad=2))
+    out = attn(b.dev(b.q), b.dev(b.kc), b.dev(b.vc), *b.index()).double().cpu()
+    bad = torch.zeros(b.T, dtype=torch.bool)
+    bad[600] = True   # the row of the last position
+    bad[620:749] = True  # (the first of the 130 rows sees nothing)
+    assert torch.isnan(out[bad]).all()
+    good = ~bad
+    good[0] = good[749:] = False
+    assert ((out - want).abs()[good] <= tol[good]).all() and (out[619] == 0).all()
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -84,9 +120,10 @@ def test_attention_many_sequences(gpu, B):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-def test_attention_rows_that_see_nothing(gpu, dtype):
+@LONG
+def test_attention_rows_that_see_nothing(gpu, dtype, long):
     """Fewer cached tokens than rows: the first rows' positions are below zero."""
-    b = po.Batch([5, 150, 1, 40], [2, 30, 0, -3], 8, 2, 128, 16, dtype, seed=3, lead=2, pad=2)
+    b = po.Batch([5, 150, 1, 40], [2, 30, 0, -3], 8, 2, 128, 16, dtype, seed=3, lead=2, pad=2, slack=_slack(long, 16))
     out = _check_attn(b, "empty rows")
     assert (out[2:5] == 0).all() and (out[5] != 0).any()
 
@@ -94,9 +131,10 @@ def test_attention_rows_that_see_nothing(gpu, dtype):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("heads,kv_heads,D,page", [(8, 2, 128, 16), (4, 4, 64, 64), (2, 1, 40, 8)])
 @pytest.mark.parametrize("chunks,lens", [([50, 1], [200, 700]), ([300], [1300])])
-def test_attention_garbage_beside_the_keys(gpu, dtype, heads, kv_heads, D, page, chunks, lens):
+@LONG
+def test_attention_garbage_beside_the_keys(gpu, dtype, heads, kv_heads, D, page, chunks, lens, long):
     """NaN and infinities in later tokens' keys and values, in slots past the end and in unused pages."""
-    b = po.Batch(chunks, lens, heads, kv_heads, D, page, dtype, seed=11)
+    b = po.Batch(chunks, lens, heads, kv_heads, D, page, dtype, seed=11, slack=_slack(long, page))
     # the last new token of the first sequence is NaN / inf: rows before it must not see it
     pos = lens[0] - 1
     b.kc[int(b.table[0, pos // page]), :, pos % page] = float("nan")
@@ -118,9 +156,10 @@ def test_attention_garbage_beside_the_keys(gpu, dtype, heads, kv_heads, D, page,
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("D", [64, 128, 24])
-def test_attention_infinite_values(gpu, dtype, D):
+@LONG
+def test_attention_infinite_values(gpu, dtype, D, long):
     """An infinite V entry that a row sees makes that dim infinite, and no other dim or row."""
-    b = po.Batch([40, 1], [100, 300], 4, 2, D, 16, dtype, seed=2, spread=0.5)
+    b = po.Batch([40, 1], [100, 300], 4, 2, D, 16, dtype, seed=2, spread=0.5, slack=_slack(long, 16))
     b.vc[int(b.table[0, 80 // 16]), 1, 80 % 16, 3] = float("inf")
     out = attn(b.dev(b.q), b.dev(b.kc), b.dev(b.vc), *b.index()).double().cpu()
     b.vc[int(b.table[0, 80 // 16]), 1, 80 % 16, 3] = 0.0
@@ -134,9 +173,10 @@ def test_attention_infinite_values(gpu, dtype, D):
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("D,page", [(128, 16), (64, 32), (20, 8)])
 @pytest.mark.parametrize("entry", [-1, 1 << 30, -(1 << 31), "pages"])
-def test_attention_pages_outside_the_cache(gpu, dtype, D, page, entry):
+@LONG
+def test_attention_pages_outside_the_cache(gpu, dtype, D, page, entry, long):
     """Rows that see such a page are NaN, the others are not."""
-    b = po.Batch([90, 1, 1], [200, 200, 600], 4, 2, D, page, dtype, seed=4)
+    b = po.Batch([90, 1, 1], [200, 200, 600], 4, 2, D, page, dtype, seed=4, slack=_slack(long, page))
     want, tol = po.attention(b)
     at = 160 // page * page
     b.table[0, at // page] = b.pages if entry == "pages" else entry
@@ -163,9 +203,10 @@ def test_attention_longer_than_the_table(gpu, dtype):
 
 
 @pytest.mark.parametrize("starts", [[0, 9, 4, 20], [5, 3, 2, 1], [-4, 2, 1 << 30, 7], [20, 20, 20, 20]])
-def test_attention_starts_that_do_not_rise(gpu, starts):
+@LONG
+def test_attention_starts_that_do_not_rise(gpu, starts, long):
     """Refused by no check (the host does not read them): any result, but no access outside the buffers."""
-    b = po.Batch([5, 5, 10], [50, 90, 20], 4, 2, 64, 16, BF16, seed=6)
+    b = po.Batch([5, 5, 10], [50, 90, 20], 4, 2, 64, 16, BF16, seed=6, slack=_slack(long, 16))
     attn(b.dev(b.q), b.dev(b.kc), b.dev(b.vc), b.table.cuda(), torch.tensor(starts, dtype=torch.int32).cuda(),
          b.lens_t.cuda())
     torch.cuda.synchronize()
@@ -527,9 +568,11 @@ def test_attention_large_chunks(gpu, dtype, heads, kv_heads, D, page, chunks, le
     assert torch.equal(_bits(out), _bits(attn(q, kc, vc, table, starts, ln)))
 
 
-def test_attention_a_sequence_alone_or_in_a_batch(gpu):
+@LONG
+def test_attention_a_sequence_alone_or_in_a_batch(gpu, long):
     """Chunks beside single tokens (both tile sizes in one launch): each sequence within its own bound."""
-    b = po.Batch([1, 200, 16, 17, 1, 65, 64, 1], [700, 1000, 16, 300, 1, 65, 2000, 64], 8, 2, 128, 16, BF16, seed=2, pad=5)
+    b = po.Batch([1, 200, 16, 17, 1, 65, 64, 1], [700, 1000, 16, 300, 1, 65, 2000, 64], 8, 2, 128, 16, BF16, seed=2, pad=5,
+                 slack=_slack(long, 16))
     _check_attn(b, "mixed")
-    b = po.Batch([1, 200, 64, 65, 1, 130, 1], [700, 1000, 64, 300, 1, 130, 64], 4, 4, 64, 8, F16, seed=3, pad=1)
+    b = po.Batch([1, 200, 64, 65, 1, 130, 1], [700, 1000, 64, 300, 1, 130, 64], 4, 4, 64, 8, F16, seed=3, pad=1, slack=_slack(long, 8))
     _check_attn(b, "mixed")

@@ -8,19 +8,21 @@ import random
 
 import pytest
 
-SLICE, MIN_SLICED, SPLIT_ROWS = 256, 1536, 64
+SLICE, MIN_SLICED, SPLIT_ROWS, TILED_ROWS, ONE_EACH = 256, 1536, 16, 64, 256
 
 
 def plan(T, B, Hq, Hk, page, width, fast, tiles_ok):
     """(rows a tile, items, target) of both classes, as pa_plan."""
     G, rows, seqs = Hq // Hk, T * (Hq // Hk), min(B, T)
-    tiles = fast and tiles_ok and page % 16 == 0 and rows > SPLIT_ROWS
+    sliced = page * width > MIN_SLICED
+    tiles = fast and tiles_ok and page % 16 == 0 and rows > SPLIT_ROWS and (
+        T > B or rows > TILED_ROWS if sliced else (rows // 16 + seqs // 2) * Hk > 2 * ONE_EACH)
     bm = [16 if fast else 4, 128]
     items, target = [(rows // bm[0] + seqs) * Hk, 0], [0, 0]
     if tiles:
-        items[0] = min(items[0], seqs * (SPLIT_ROWS // bm[0]) * Hk)
+        items[0] = min(items[0], seqs * -(-SPLIT_ROWS // bm[0]) * Hk)
         items[1] = (rows // 128 + min(seqs, rows // (SPLIT_ROWS + 1))) * Hk
-    if page * width > MIN_SLICED:
+    if sliced:
         target[0] = 1536
         if tiles and rows // 128 * Hk < 4 * 512:
             target[1] = 512
