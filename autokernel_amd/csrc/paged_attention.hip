@@ -839,7 +839,7 @@ __device__ __forceinline__ void pa_rows_f32_item(const PaArgs& a, uint32_t item,
 //   * No pass over what a row does not see: V of masked keys only has to be finite. Where a row's result is
 //     NaN, or a page lies outside the cache, the item's rows are computed again by pa_row.
 // Bound by the MFMA and the softmax VALU work, as fa_fwd2 is. 512 tokens after 16001 (32 heads of 128, 8 KV heads,
-// bf16): 156 us, 875 TFLOP/s, MFMA busy 41 % of the time, half of it waiting; four prompts of 2048: 167 to 186 us, 740
+// bf16): 156 us, 875 TFLOP/s, MFMA busy 40 % of the time, half of it waiting; four prompts of 2048: 167 to 186 us, 740
 // to 820. A prompt of 8192 runs at 992 TFLOP/s, fa_fwd2 on dense keys at 1074.
 constexpr int kPtRows = 32 * kPaWaves;
 
