@@ -43,7 +43,7 @@ def _slack(long, page):
     return 1600 // page + 1 if long else 1
 
 
-SHAPES = [(8, 2, 128), (4, 4, 64), (6, 2, 64), (32, 2, 128), (3, 1, 80), (5, 5, 17), (4, 2, 256), (16, 1, 128), (2, 1, 1)]
+SHAPES = [(8, 2, 128), (40, 1, 64), (4, 4, 64), (6, 2, 64), (32, 2, 128), (3, 1, 80), (5, 5, 17), (4, 2, 256), (16, 1, 128), (2, 1, 1)]
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
