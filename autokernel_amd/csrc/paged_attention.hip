@@ -276,7 +276,7 @@ __device__ void pa_one_by_one(const PaArgs& a, const PaItem& it, int r_begin, in
 }
 
 // Any type, head_dim and alignment: one wave per row, four rows per block. Each row reads its keys for itself, from the
-// L2 where rows share them (64 ragged sequences of 200 to 8000 tokens: 1391 us, 130 by pa_rows).
+// L2 where rows share them (64 ragged sequences of 200 to 8000 tokens: 1391 us, 120 by pa_rows).
 constexpr int kPaRowTile = kPaWaves;
 template <typename T>
 __global__ __launch_bounds__(kPaThreads) void pa_general(const PaArgs a) {
@@ -448,8 +448,8 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
 //   * Weights are rounded to the element type for the product; the sum adds the rounded ones.
 // Keys past a row's position weigh nothing as long as their V is finite. Where a result is NaN, or a page
 // lies outside the cache, the rows are computed again by pa_row.
-// 64 sequences of 200 to 8000 cached tokens, one new one each, 8 KV heads of 128 in bf16: 613 MB in 120 us, 5.1 TB/s (a
-// large copy moves as much), and 7.5 for the merge. One sequence of 1000: 14.4 us, eight CUs' latency: 1 us to find
+// 64 sequences of 200 to 8000 cached tokens, one new one each, 8 KV heads of 128 in bf16: 613 MB in 110 us, 5.6 TB/s (a
+// large copy moves 5.1, a large read 6.1), and 7 for the merge. One sequence of 1000: 14.4 us, eight CUs' latency: 1 us to find
 // the item, 2 to its page numbers and 3 per two steps of keys.
 constexpr int kPrRows = 16, kPrKeys = 32;
 struct PrMaximum {
@@ -547,7 +547,16 @@ __device__ __forceinline__ void pr_finish(const PaArgs& a, const PaItem& it, PrS
   }
 }
 
-template <typename T, int D, int PG, int NW>
+// A piece of a K or V row. STREAM: nontemporal, for keys that no other block reads (64 ragged sequences 129.5 ->
+// 120.6 us a call; 256 x 4000 tokens 711 -> 649; 40 x 1600 after a flush of the caches 72 -> 68, but 56 -> 63 where the
+// last call's keys are still in them).
+template <bool STREAM, typename V>
+__device__ __forceinline__ V pr_load(const uint16_t* p) {
+  if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+  else return *reinterpret_cast<const V*>(p);
+}
+
+template <typename T, int D, int PG, int NW, bool STREAM>
 __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrShared<D, NW>& sh) {
   constexpr int NS = D / 32, VW = D / 16;
   constexpr int NK = PG == 8 ? 1 : 2, NV = PG == 8 ? 1 : 8;  // page numbers of a lane and step
@@ -601,7 +610,7 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
       bad |= !in;
       const uint16_t* src = Kb + (in ? pg * a.kcp + slot * a.kct : 0);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) st.k[t][s] = in ? ld16(src + s * 32) : u32x4{0u, 0u, 0u, 0u};
+      for (int s = 0; s < NS; ++s) st.k[t][s] = in ? pr_load<STREAM, u32x4>(src + s * 32) : u32x4{0u, 0u, 0u, 0u};
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -610,7 +619,7 @@ __device__ __forceinline__ void pa_rows_item(const PaArgs& a, uint32_t item, PrS
       const bool in = (uint32_t)pg < a.s.num_pages && (!tail || key < kend);
       const uint32_t slot = (uint32_t)key - fdiv((uint32_t)key, a.s.page_div) * a.s.page_size;
       if (in) {
-        st.v[e] = *reinterpret_cast<const VV*>(Vb + pg * a.vcp + slot * a.vct);
+        st.v[e] = pr_load<STREAM, VV>(Vb + pg * a.vcp + slot * a.vct);
       } else {
 #pragma unroll
         for (int x = 0; x < VW / 2; ++x) st.v[e][x] = 0u;
@@ -1180,11 +1189,11 @@ __device__ __forceinline__ void pa_tiles_item(const PaArgs& a, uint32_t item, Pt
     }
 }
 
-template <typename T, int D, int PG, int NW>
+template <typename T, int D, int PG, int NW, bool STREAM>
 __global__ __launch_bounds__(NW* kWave, 2) void pa_rows(const PaArgs a) {
   __shared__ __attribute__((aligned(16))) PrShared<D, NW> sh;
   if constexpr (T::kCode == AK_F32) pa_rows_f32_item<D, PG == 8 ? 4 : 1, NW>(a, blockIdx.x, sh);
-  else pa_rows_item<T, D, PG, NW>(a, blockIdx.x, sh);
+  else pa_rows_item<T, D, PG, NW, STREAM>(a, blockIdx.x, sh);
 }
 // Both classes in one launch: the blocks of the large tiles first.
 template <typename T, int D>
@@ -1194,13 +1203,14 @@ __global__ __launch_bounds__(kPaThreads, 2) void pa_mixed(const PaArgs a) {
     PrShared<D, kPaWaves> r;
   } sh;
   if (blockIdx.x < a.c[1].items) pa_tiles_item<T, D>(a, blockIdx.x, sh.t);
-  else pa_rows_item<T, D, 8, kPaWaves>(a, blockIdx.x - a.c[1].items, sh.r);
+  else pa_rows_item<T, D, 8, kPaWaves, true>(a, blockIdx.x - a.c[1].items, sh.r);
 }
 
 // What a call launches: the most items of each class and their partials. Keys are sliced only where some
 // sequence can be longer than kPaMinSliced, below which the merge costs what the shorter walk saves (one
 // sequence of 1000 keys: 5 us each).
-// Items aimed at: 1536 tiles of 16 rows (64 ragged sequences 128.6 us; 512: 135.8, 1024: 131, 2048: 131.4), 512 of 128
+// Items aimed at: 1536 tiles of 16 rows (64 ragged sequences, before keys were streamed, 128.6 us; 512: 135.8, 1024:
+// 131, 2048: 131.4), 512 of 128
 // rows (512 tokens after 16001 157 us; 1024: 172).
 // A sequence of more rows than one tile of 16 takes tiles of 128, which read its keys once (64 sequences over 2000
 // tokens, 32 / 64 rows each: 103 / 109 us, in tiles of 16: 179 / 204), in calls where that pays:
@@ -1259,7 +1269,7 @@ template <typename T, int BM0, int BM1, int JN>
 static void pa_launch_merge(PaArgs& a, hipStream_t st) {
   if (a.c[0].target <= 0.f && a.c[1].target <= 0.f) return;
   const int64_t rows = (int64_t)a.s.T * a.Hq;
-  // 64 tokens of 32 heads, up to 7 slices: the whole call 129.6 us with a group per row, 132.0 with a block
+  // 64 tokens of 32 heads, up to 7 slices: a block per row costs the call 2.4 us more than a group
   const bool wide = rows < 1024;
   a.f_units = make_fastdiv((uint32_t)(wide ? a.Hq : (a.Hq + 3) / 4));
   // where only sequences with few rows may be sliced, blocks for as many rows as these can have
@@ -1276,12 +1286,23 @@ static int launch_general(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
   return record_launch();
 }
 // Blocks of eight waves where a batch has at most one per CU: each wave walks half as many keys (one sequence of
-// 1000: 14.4 us, 15.8 with four). With more blocks than that four waves share a CU with three other blocks.
+// 1000: 14.4 us, 15.8 with four). With more blocks than that four waves leave room for a second one on the CU.
+// Single tokens over long caches stream their keys (16 over 8000: 105 -> 97 us); fp32 keys, which take several loads per
+// 128 bytes, do not (210 -> 375).
 template <typename T, int D, int PG>
 static void launch_rows(const PaArgs& a, const PaPlan& p, hipStream_t st) {
   const dim3 grid((unsigned)p.items[0]);
-  if (p.items[0] <= kPaOneEach) pa_rows<T, D, PG, 8><<<grid, 8 * kWave, 0, st>>>(a);
-  else pa_rows<T, D, PG, kPaWaves><<<grid, kPaThreads, 0, st>>>(a);
+  if (p.items[0] <= kPaOneEach) {
+    pa_rows<T, D, PG, 8, false><<<grid, 8 * kWave, 0, st>>>(a);
+    return;
+  }
+  if constexpr (T::kCode != AK_F32) {
+    if (p.target[0] > 0 && a.s.T <= a.s.B) {
+      pa_rows<T, D, PG, kPaWaves, true><<<grid, kPaThreads, 0, st>>>(a);
+      return;
+    }
+  }
+  pa_rows<T, D, PG, kPaWaves, false><<<grid, kPaThreads, 0, st>>>(a);
 }
 template <typename T, int D>
 static int launch_fast(PaArgs a, const PaPlan& p, void* ws, hipStream_t st) {
