@@ -111,6 +111,17 @@ def test_attention_sliced(gpu, dtype, heads, kv_heads, D):
     _check_attn(b, "sliced")
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,D,page", [(8, 2, 128, 16), (12, 4, 64, 24), (2, 2, 64, 8), (32, 2, 128, 32), (4, 2, 96, 16)])
+@pytest.mark.parametrize("B", [6, 40])
+def test_attention_single_tokens_sliced(gpu, dtype, heads, kv_heads, D, page, B):
+    """Decode steps over long and short caches, a sequence without a new token among them, with few rows and with many."""
+    g = torch.Generator().manual_seed(B + D)
+    lens = [2600, 1, 257, 0, 513, 1537] + torch.randint(1, 1200, (B - 6,), generator=g).tolist()
+    b = po.Batch([1, 1, 1, 0, 1, 1] + [1] * (B - 6), lens, heads, kv_heads, D, page, dtype, seed=B, pad=1)
+    _check_attn(b, "single tokens")
+
+
 @pytest.mark.parametrize("B", [63, 64, 65, 130, 300])
 def test_attention_many_sequences(gpu, B):
     g = torch.Generator().manual_seed(B)

@@ -96,6 +96,15 @@ def test_widths(gpu, dt, V):
 
 
 @pytest.mark.parametrize("dt", DT)
+def test_largest_vocabulary(gpu, dt):
+    # (min_p where the margin of 1e-9 is one: around a weight of 1e-6 it spans 0.002 of x, which holds some hundred of a
+    # million elements; around 0.02 it spans 1e-7)
+    x, u = zipf(3, 1 << 20, dt, 6, a=1.1)
+    for kw in (dict(), dict(top_p=0.8), dict(top_k=100), dict(top_k=100000, min_p=0.02), dict(temperature=0.0)):
+        check(x, u, "largest", **kw)
+
+
+@pytest.mark.parametrize("dt", DT)
 def test_rows_of_their_own(gpu, dt):
     R = 90
     x, u = zipf(R, 3001, dt, 5)
