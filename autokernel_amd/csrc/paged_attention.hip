@@ -64,7 +64,8 @@ __device__ __forceinline__ PaSeq pa_seq(const PagedSeqs& s, int b) {
 }
 
 struct PaItem {
-  int b, hk, tile, split, nsplit, chunk;
+  int b, hk, tile, split, nsplit;
+  int chunk;      // keys of a slice of this sequence
   uint32_t slot;  // the item's place among its class's partials
   PaSeq seq;
 };
@@ -81,9 +82,9 @@ __device__ __forceinline__ int pa_wave_scan(int v) {
   return v;
 }
 
-// Keys per slice: all of them when the class's work fills the chip without slicing, else the work over
-// `target`, in multiples of kPaSlice.
-constexpr int kPaSlice = 256;
+// Keys per slice, at most: all of them when the class's work fills the chip without slicing, else the work over
+// `target`, in multiples of kPaSlice. A sequence's slices are alike, in multiples of kPaStep.
+constexpr int kPaSlice = 256, kPaStep = 128;
 template <int BM, int CLS>
 __device__ __forceinline__ int pa_tiles_of(const PaArgs& a, const PaSeq& q) {
   const int rows = q.n * a.G;
@@ -105,14 +106,25 @@ __device__ __forceinline__ void pa_each(const PaArgs& a, const PaBatch& x, F f) 
 }
 template <int BM, int CLS>
 __device__ __forceinline__ int pa_chunk(const PaArgs& a, const PaBatch& x) {
-  if (a.c[CLS].target <= 0.f) return INT_MAX;
-  float w = 0.f;
+  float target = a.c[CLS].target;
+  if (target <= 0.f) return INT_MAX;
+  float w = 0.f, tiles = 0.f, longest = 0.f;
   pa_each(a, x, [&](int, const PaSeq& q) {
-    w += (float)pa_tiles_of<BM, CLS>(a, q) * (float)q.len;
+    const float n = (float)pa_tiles_of<BM, CLS>(a, q), len = (float)q.len;
+    w += n * len;
+    if constexpr (CLS == 0) {
+      tiles += n;
+      longest = n > 0.f ? fmaxf(longest, len) : longest;
+    }
     return false;
   });
-  w = wave_sum(w) * (float)a.Hk * 1.001f;
-  const float c = ceilf(w / a.c[CLS].target / (float)kPaSlice) * (float)kPaSlice;
+  w = wave_sum(w);
+  // Sequences of about one length balance by themselves, and two rounds of items are enough (128 of 2000 tokens 180 us in
+  // three, 170 in two; 24 of 3000 65, 61); ragged ones not (64 of 200 to 8000 120.4 in three, 123.2 in two).
+  if constexpr (CLS == 0)
+    if (wave_max(longest) * wave_sum(tiles) < 1.5f * w) target *= 2.f / 3.f;
+  w *= (float)a.Hk * 1.001f;
+  const float c = ceilf(w / target / (float)kPaSlice) * (float)kPaSlice;
   return pa_uniform(c >= 1e9f ? INT_MAX : max((int)c, kPaSlice));
 }
 __device__ __forceinline__ int pa_splits(int len, int chunk) { return len > 0 ? (len - 1) / chunk + 1 : 1; }
@@ -145,6 +157,9 @@ __device__ __forceinline__ bool pa_find(const PaArgs& a, uint32_t it, PaItem& o)
     o.seq.len = __builtin_amdgcn_readlane(q.len, l);
     o.seq.overlong = __builtin_amdgcn_readlane((int)q.overlong, l) != 0;
     o.nsplit = __builtin_amdgcn_readlane(splits, l);
+    // equal slices: 2000 keys are two of 1024, not 1536 and 464 (128 such sequences:
+    // 228 us, 180 in equal ones)
+    if (o.nsplit > 1) o.chunk = pa_uniform((((o.seq.len - 1) / o.nsplit + 1) + kPaStep - 1) / kPaStep * kPaStep);
     const uint32_t rel = it - base - (uint32_t)__builtin_amdgcn_readlane(inc - cnt, l);
     const uint32_t y = fdiv(rel, a.f_hk);
     o.hk = pa_uniform((int)(rel - y * a.Hk));
@@ -1209,8 +1224,8 @@ __global__ __launch_bounds__(kPaThreads, 2) void pa_mixed(const PaArgs a) {
 // What a call launches: the most items of each class and their partials. Keys are sliced only where some
 // sequence can be longer than kPaMinSliced, below which the merge costs what the shorter walk saves (one
 // sequence of 1000 keys: 5 us each).
-// Items aimed at: 1536 tiles of 16 rows (64 ragged sequences, before keys were streamed, 128.6 us; 512: 135.8, 1024:
-// 131, 2048: 131.4), 512 of 128
+// Items aimed at: 1536 tiles of 16 rows (64 ragged sequences 120.4 us; 1024: 123.2, 2048: 120.9; two thirds for
+// sequences of about one length, see pa_chunk), 512 of 128
 // rows (512 tokens after 16001 157 us; 1024: 172).
 // A sequence of more rows than one tile of 16 takes tiles of 128, which read its keys once (64 sequences over 2000
 // tokens, 32 / 64 rows each: 103 / 109 us, in tiles of 16: 179 / 204), in calls where that pays:

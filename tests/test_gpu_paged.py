@@ -265,7 +265,7 @@ def test_attention_positions_up_to_2_31(gpu, width):
     """Nearly 2^31 cached tokens: one page over and over (scores 0, values 1) and a last one with scores of 13.125 and
     values of -1, which carries half of the weight. Sums of ones are exact to 2^24, and what is added up of slices
     and exponentials rounds a few thousand times at 2^-24: below 1e-3 / 4 with the share of bf16 weights (2^-8 of
-    the last slice's 1 / 1500)."""
+    the last slice's 1 / 1000)."""
     page, D = 4096, 64
     kc = torch.zeros(2, 1, page, D, dtype=BF16, device="cuda")
     vc = torch.ones_like(kc)

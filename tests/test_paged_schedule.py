@@ -8,7 +8,7 @@ import random
 
 import pytest
 
-SLICE, MIN_SLICED, SPLIT_ROWS, TILED_ROWS, ONE_EACH = 256, 1536, 16, 64, 256
+SLICE, STEP, MIN_SLICED, SPLIT_ROWS, TILED_ROWS, ONE_EACH = 256, 128, 1536, 16, 64, 256
 
 
 def plan(T, B, Hq, Hk, page, width, fast, tiles_ok):
@@ -47,7 +47,10 @@ def f32(x):
 def chunk(seqs, G, Hk, bm, mine, target):
     if target == 0:
         return None
-    w = f32(sum(f32(-(-s.n * G // bm)) * f32(s.len) for s in seqs if mine(s)) * Hk * 1.001)
+    w = f32(sum(f32(-(-s.n * G // bm)) * f32(s.len) for s in seqs if mine(s)))
+    if bm < 128 and max([s.len for s in seqs if mine(s)] + [0]) * sum(-(-s.n * G // bm) for s in seqs if mine(s)) < 1.5 * w:
+        target = f32(target * 2 / 3)  # sequences of about one length
+    w = f32(w * Hk * 1.001)
     c = -(-int(w / target) // SLICE) * SLICE if w / target == int(w / target) else (int(w / target) // SLICE + 1) * SLICE
     return max(c, SLICE)
 
@@ -89,9 +92,11 @@ def check(chunks, lens, Hq, Hk, D, page, width, fast, tiles_ok=True, starts=None
             assert len(set(items)) == len(items)
         for b, hk, tile, sp in items[:planned[cls]]:
             s = seqs[b]
-            lo = 0 if c is None or splits(s.len, c) == 1 else sp * c
-            hi = min(max(0, s.len - s.n + min(s.n * G - 1, tile * bm[cls] + bm[cls] - 1) // G + 1),
-                     s.len if splits(s.len, c) == 1 else lo + c)
+            n = splits(s.len, c)
+            each = -(-(-(-s.len // n)) // STEP) * STEP if n > 1 else s.len  # keys of this sequence's slices
+            lo = sp * each
+            hi = min(max(0, s.len - s.n + min(s.n * G - 1, tile * bm[cls] + bm[cls] - 1) // G + 1), lo + each)
+            assert n * each >= s.len and lo < 2 ** 31 and (n == 1 or each <= c)
             assert 0 <= tile * bm[cls] < s.n * G and hi <= s.len <= page * width
             if hi > lo:
                 assert (hi - 1) // page < width
