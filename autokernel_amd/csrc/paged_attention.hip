@@ -414,8 +414,11 @@ __global__ __launch_bounds__(kPaThreads) void pa_merge(const PaArgs a) {
         const int d = 64 * j + 4 * c;
         float* y = sum.acc[j];
         if constexpr (JN <= 2) {  // head_dim 64 JN, aligned rows
-          if constexpr (T::kCode == AK_F32) *reinterpret_cast<f32x4*>(o + d) = f32x4{y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
-          else *reinterpret_cast<u32x2*>(o + d) = u32x2{fa2_pack<T>(y[0] * inv, y[1] * inv), fa2_pack<T>(y[2] * inv, y[3] * inv)};
+          if constexpr (T::kCode == AK_F32)
+            *reinterpret_cast<f32x4*>(o + d) = f32x4{y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+          else
+            *reinterpret_cast<u32x2*>(o + d) =
+                u32x2{fa2_pack<T>(y[0] * inv, y[1] * inv), fa2_pack<T>(y[2] * inv, y[3] * inv)};
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)

@@ -262,8 +262,8 @@ def kv_append(q_out: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.
     T, Hkv, D = k.shape
     rows, rot = (0, 0) if cos is None else (cos.shape[0], 2 * cos.shape[1])
     qs, os = (_NO_STRIDES, _NO_STRIDES) if q is None else (_strides(q.stride()), _strides(q_out.stride()))
-    _run("ak_kv_append", k, None, _code(k, "kv_append"), _lib.ptr(q), k.data_ptr(), v.data_ptr(), _lib.ptr(q_out), k_cache.data_ptr(),
-         v_cache.data_ptr(), _lib.ptr(cos), _lib.ptr(sin), page_table.data_ptr(), q_starts.data_ptr(),
+    _run("ak_kv_append", k, None, _code(k, "kv_append"), _lib.ptr(q), k.data_ptr(), v.data_ptr(), _lib.ptr(q_out),
+         k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(cos), _lib.ptr(sin), page_table.data_ptr(), q_starts.data_ptr(),
          kv_lens.data_ptr(), T, kv_lens.shape[0], 0 if q is None else q.shape[1], Hkv, D, rot, rows,
          *_paged_sizes(k_cache, page_table), qs, _strides(k.stride()), _strides(v.stride()), os,
          _strides(k_cache.stride()), _strides(v_cache.stride()), int(bool(interleaved)))
@@ -284,8 +284,8 @@ def paged_attn(o: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, v_cache:
     # fp32 partials of key slices
     nbytes = _paged_workspace_bytes(code, T, B, Hq, Hkv, D, sizes[1], sizes[2])
     ws = torch.empty(nbytes // 4, device=q.device, dtype=torch.float32) if nbytes > 0 else None
-    _run("ak_paged_attn", q, None, code, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), page_table.data_ptr(),
-         q_starts.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, *sizes, _strides(q.stride()),
+    _run("ak_paged_attn", q, None, code, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(),
+         page_table.data_ptr(), q_starts.data_ptr(), kv_lens.data_ptr(), T, B, Hq, Hkv, D, *sizes, _strides(q.stride()),
          _strides(k_cache.stride()), _strides(v_cache.stride()), _strides(o.stride()), sm_scale, _lib.ptr(ws), nbytes)
 
 
