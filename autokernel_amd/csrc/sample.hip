@@ -24,7 +24,7 @@
 // What bounds sm_any: the 64-bit weights of a whole row where no top-k spares them, about 25 instructions an
 // element. So everything else an element meets is one or two comparisons: a bin, or min-p, is a range of
 // floats, whose end is found once per row by trying 64 candidates at a time.
-// 64 rows of 50257 fp32 with settings of all kinds: 35 us, of which 4 read the row; the slowest rows are those with
+// 64 rows of 50257 fp32 with settings of all kinds: 33 to 42 us, of which 4 read the row; the slowest rows are those with
 // top-p alone (28 us for 131072 weights, 16 with a constant in place of the weight, and 28 without the atomics).
 #include <float.h>
 #include <limits.h>
